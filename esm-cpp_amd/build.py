@@ -23,8 +23,8 @@ OBJDIR = os.path.join(HERE, "_build")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB = os.path.join(LIBDIR, "libesm_gfx950.so")
 
-SOURCES = ["gemm_i8.hip", "attention.hip", "elementwise.hip", "gemm_f32.hip", "x86_exact.hip", "capi.cpp", "gguf.cpp",
-           "observer.cpp"]
+SOURCES = ["gemm_i8.hip", "attention.hip", "elementwise.hip", "gemm_f32.hip", "x86_exact.hip", "linear_i4.hip",
+           "block_attention.hip", "capi.cpp", "gguf.cpp", "observer.cpp"]
 # Per-file flags: the reference's x86 kernels are restated with every fused
 # multiply-add spelled out, so the compiler must form no others.
 EXTRA = {"x86_exact.hip": ["-ffp-contract=off"]}

@@ -144,6 +144,12 @@ struct esm_gfx950_weight {
   float* scales = nullptr;  // [N]
 };
 
+struct esm_gfx950_weight_i4 {
+  int N = 0, K = 0, group = 0, groups = 0, tiles_k = 0;
+  uint32_t* codes = nullptr;  // linear_i4_layout's order
+  float* scales = nullptr;
+};
+
 // Activation observer (reference esm::ActivationObserver): per-site
 // reservoirs on the host, plus device and pinned staging for the gathered
 // values, grown on demand (kReservoirSize entries per site of one call).
@@ -871,6 +877,337 @@ extern "C" int esm_gfx950_attention_varlen_bf16(esm_gfx950_ctx* ctx, const uint1
   ESM_HIP(ctx, launch_attention_mfma(q, k, v, 0, v_is_fp16 ? 0 : 1, ld, d_cu, d_work, nwork, out, ld, nullptr,
                                      ctx->stream));
   ESM_TRY(ctx->time_end(slot));
+  return ESM_GFX950_OK;
+}
+
+// ------------------------------------------------------------ 4-bit linears
+namespace {
+// Makes the context's device the current one for a call, and the caller's again
+// afterwards.
+struct DeviceScope {
+  int before = -1;
+  explicit DeviceScope(const esm_gfx950_ctx* ctx) {
+    int d = -1;
+    if (hipGetDevice(&d) == hipSuccess && d != ctx->device && hipSetDevice(ctx->device) == hipSuccess) before = d;
+  }
+  ~DeviceScope() {
+    if (before >= 0) hipSetDevice(before);
+  }
+};
+
+int elem_size(int dtype) { return dtype == ESM_GFX950_F32 ? 4 : dtype == ESM_GFX950_F16 || dtype == ESM_GFX950_BF16 ? 2 : 0; }
+
+// Whether [a, a + na) and [b, b + nb) bytes share memory.
+bool bytes_overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na && nb && x < y + nb && y < x + na;
+}
+
+bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// Bytes from the first to the last element of `rows` rows of `cols` elements.
+size_t span_bytes(size_t rows, size_t ld, size_t cols, size_t elem) {
+  return rows ? ((rows - 1) * ld + cols) * elem : 0;
+}
+}  // namespace
+
+extern "C" int esm_gfx950_weight_upload_i4(esm_gfx950_ctx* ctx, const uint8_t* packed, const float* scales, int N,
+                                           int K, int group, esm_gfx950_weight_i4** out) {
+  if (!ctx || !out) return ESM_GFX950_INVALID_ARGUMENT;
+  *out = nullptr;
+  ESM_REQUIRE(ctx, packed && scales && N > 0 && K > 0, "weight_upload_i4: bad arguments");
+  ESM_REQUIRE(ctx, group == 32 || group == 64 || (group > 0 && group % 128 == 0),
+              "weight_upload_i4: group must be 32, 64 or a multiple of 128");
+  // 2^40 padded codes (512 GB) are past every device.
+  const size_t tiles_n = (static_cast<size_t>(N) + 15) / 16, tiles_k = (static_cast<size_t>(K) + 127) / 128;
+  ESM_REQUIRE(ctx, tiles_n <= (size_t{1} << 29) / tiles_k, "weight_upload_i4: N x K is too large");
+  DeviceScope on(ctx);
+  esm_gfx950_weight_i4* w = nullptr;
+  try {
+    w = new esm_gfx950_weight_i4();
+    w->N = N;
+    w->K = K;
+    w->group = group;
+    w->groups = (K - 1) / group + 1;
+    w->tiles_k = static_cast<int>(tiles_k);
+    std::vector<uint32_t> codes(tiles_n * tiles_k * 256);
+    std::vector<float> s(tiles_n * 16 * w->groups);
+    linear_i4_layout(packed, scales, N, K, group, codes.data(), s.data());
+    hipError_t e = hipMalloc(&w->codes, codes.size() * 4);
+    if (e == hipSuccess) e = hipMalloc(&w->scales, s.size() * 4);
+    if (e == hipSuccess)
+      e = hipMemcpyAsync(w->codes, codes.data(), codes.size() * 4, hipMemcpyHostToDevice, ctx->stream);
+    if (e == hipSuccess) e = hipMemcpyAsync(w->scales, s.data(), s.size() * 4, hipMemcpyHostToDevice, ctx->stream);
+    const hipError_t done = hipStreamSynchronize(ctx->stream);
+    if (e == hipSuccess) e = done;
+    if (e != hipSuccess) {
+      if (w->codes) hipFree(w->codes);
+      if (w->scales) hipFree(w->scales);
+      delete w;
+      return ctx->hip_fail("weight_upload_i4", e);
+    }
+  } catch (const std::exception& e) {
+    delete w;
+    return ctx->fail(ESM_GFX950_INTERNAL, std::string("weight_upload_i4: ") + e.what());
+  }
+  *out = w;
+  return ESM_GFX950_OK;
+}
+
+extern "C" int esm_gfx950_weight_free_i4(esm_gfx950_ctx* ctx, esm_gfx950_weight_i4* w) {
+  if (!ctx) return ESM_GFX950_INVALID_ARGUMENT;
+  if (!w) return ESM_GFX950_OK;
+  DeviceScope on(ctx);
+  ESM_HIP(ctx, hipStreamSynchronize(ctx->stream));
+  hipFree(w->codes);
+  hipFree(w->scales);
+  delete w;
+  return ESM_GFX950_OK;
+}
+
+extern "C" int esm_gfx950_linear_i4(esm_gfx950_ctx* ctx, const void* A, int lda, const esm_gfx950_weight_i4* W,
+                                    const float* bias, void* C, int ldc, int M, int N, int K, int dtype) {
+  if (!ctx) return ESM_GFX950_INVALID_ARGUMENT;
+  const int size = elem_size(dtype);
+  ESM_REQUIRE(ctx, size, "linear_i4: unknown dtype");
+  ESM_REQUIRE(ctx, W && M >= 0, "linear_i4: bad arguments");
+  if (W->N != N || W->K != K)
+    return ctx->fail(ESM_GFX950_SHAPE_MISMATCH, "linear_i4: weight shape does not match N, K");
+  if (M == 0) return ESM_GFX950_OK;
+  ESM_REQUIRE(ctx, A && C, "linear_i4: null pointer");
+  ESM_REQUIRE(ctx, lda >= K && ldc >= N, "linear_i4: lda must be >= K and ldc >= N");
+  ESM_REQUIRE(ctx, aligned(A, size) && aligned(C, size) && aligned(bias, 4), "linear_i4: misaligned pointer");
+  ESM_REQUIRE(ctx, !bytes_overlap(A, span_bytes(M, lda, K, size), C, span_bytes(M, ldc, N, size)),
+              "linear_i4: C shares memory with A");
+  DeviceScope on(ctx);
+  LinearI4Args p;
+  p.A = A;
+  p.lda = lda;
+  p.W = W->codes;
+  p.scales = W->scales;
+  p.bias = bias;
+  p.C = C;
+  p.ldc = ldc;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.group = W->group;
+  p.groups = W->groups;
+  p.tiles_k = W->tiles_k;
+  p.vec_a = aligned(A, 16) && static_cast<size_t>(lda) * size % 16 == 0;
+  ESM_HIP(ctx, launch_linear_i4(p, dtype, ctx->stream));
+  return ESM_GFX950_OK;
+}
+
+// ------------------------------------------------------------ block attention
+namespace {
+// Blocks of n keys.
+int blocks_of(int n, int block_size) { return n > 0 ? (n - 1) / block_size + 1 : 0; }
+
+// Fills the table of a batch of the block attention ops: in the kernel's
+// arguments up to kInlineSeqs sequences, else copied to op scratch behind
+// `reserve` bytes (through the pinned staging up to its size). cu_q may be null
+// (block means). Returns with *reserved pointing at the scratch when reserve > 0.
+int stage_sequences(esm_gfx950_ctx* ctx, const int* cu_q, const int* cu_k, int batch, int block_size, size_t reserve,
+                    SeqTable* t, void** reserved) {
+  t->batch = batch;
+  const size_t n = static_cast<size_t>(batch) + 1;
+  std::vector<int> host;
+  int *hq = t->cu_q, *hk = t->cu_k, *hb = t->cb;
+  if (batch > kInlineSeqs) {
+    host.resize(3 * n);
+    hq = host.data();
+    hk = hq + n;
+    hb = hk + n;
+  }
+  for (size_t i = 0; i < n; ++i) {
+    hq[i] = cu_q ? cu_q[i] : 0;
+    hk[i] = cu_k[i];
+    hb[i] = i == 0 ? 0 : hb[i - 1] + blocks_of(cu_k[i] - cu_k[i - 1], block_size);
+  }
+  if (batch <= kInlineSeqs) {
+    if (reserve) ESM_TRY(ctx->get_scratch(reserve, reserved));
+    return ESM_GFX950_OK;
+  }
+  const size_t bytes = 3 * n * 4, at = align_up(reserve, 256);
+  void* s = nullptr;
+  ESM_TRY(ctx->get_scratch(at + bytes, &s));
+  *reserved = s;
+  char* dst = static_cast<char*>(s) + at;
+  t->dev = reinterpret_cast<int*>(dst);
+  if (bytes <= kOpMetaBytes) {
+    if (!ctx->meta_done) ESM_HIP(ctx, hipEventCreateWithFlags(&ctx->meta_done, hipEventDisableTiming));
+    if (!ctx->meta_host) ESM_HIP(ctx, hipHostMalloc(&ctx->meta_host, kOpMetaBytes, hipHostMallocDefault));
+    ESM_HIP(ctx, hipEventSynchronize(ctx->meta_done));
+    std::memcpy(ctx->meta_host, host.data(), bytes);
+    ESM_HIP(ctx, hipMemcpyAsync(dst, ctx->meta_host, bytes, hipMemcpyHostToDevice, ctx->stream));
+    ESM_HIP(ctx, hipEventRecord(ctx->meta_done, ctx->stream));
+    return ESM_GFX950_OK;
+  }
+  ESM_HIP(ctx, hipMemcpyAsync(dst, host.data(), bytes, hipMemcpyHostToDevice, ctx->stream));
+  ESM_HIP(ctx, hipStreamSynchronize(ctx->stream));
+  return ESM_GFX950_OK;
+}
+
+// The blocks of a batch; cu_k is non-decreasing from 0.
+size_t count_blocks(const int* cu_k, int batch, int block_size) {
+  size_t n = 0;
+  for (int b = 0; b < batch; ++b) n += blocks_of(cu_k[b + 1] - cu_k[b], block_size);
+  return n;
+}
+
+bool block_size_ok(int block_size) { return block_size >= 16 && block_size <= 1024 && block_size % 16 == 0; }
+
+// The checks that the three ops share, with their name in the messages.
+int check_block_shape(esm_gfx950_ctx* ctx, const char* op, int heads, int kv_heads, int head_dim, int block_size,
+                      int dtype) {
+  const std::string at = std::string(op) + ": ";
+  ESM_REQUIRE(ctx, elem_size(dtype), at + "unknown dtype");
+  ESM_REQUIRE(ctx, heads > 0 && kv_heads > 0 && heads % kv_heads == 0, at + "num_kv_heads must divide num_heads");
+  ESM_REQUIRE(ctx, head_dim > 0 && head_dim <= kMaxHeadDim && head_dim % 8 == 0,
+              at + "head_dim must be a multiple of 8, at most 128");
+  ESM_REQUIRE(ctx, heads <= 0x7fffffff / kMaxHeadDim, at + "too many heads");
+  ESM_REQUIRE(ctx, block_size_ok(block_size), at + "block_size must be a multiple of 16, 16..1024");
+  return ESM_GFX950_OK;
+}
+}  // namespace
+
+extern "C" int esm_gfx950_key_blocks(const int* cu_k, int batch_size, int block_size, int* cu_blocks) {
+  if (!cu_k || !cu_blocks || batch_size < 1 || !block_size_ok(block_size) || cu_k[0] != 0)
+    return ESM_GFX950_INVALID_ARGUMENT;
+  for (int b = 0; b < batch_size; ++b)
+    if (cu_k[b + 1] < cu_k[b]) return ESM_GFX950_INVALID_ARGUMENT;
+  cu_blocks[0] = 0;
+  for (int b = 0; b < batch_size; ++b)
+    cu_blocks[b + 1] = cu_blocks[b] + blocks_of(cu_k[b + 1] - cu_k[b], block_size);
+  return ESM_GFX950_OK;
+}
+
+extern "C" int esm_gfx950_key_block_means(esm_gfx950_ctx* ctx, const void* k, int ldk, const int* cu_k, int batch_size,
+                                          int num_kv_heads, int head_dim, int block_size, float* means, int dtype) {
+  if (!ctx) return ESM_GFX950_INVALID_ARGUMENT;
+  ESM_TRY(validate_batch(ctx, cu_k, batch_size, -1));
+  ESM_TRY(check_block_shape(ctx, "key_block_means", num_kv_heads, num_kv_heads, head_dim, block_size, dtype));
+  const int cols = num_kv_heads * head_dim, size = elem_size(dtype);
+  const size_t blocks = count_blocks(cu_k, batch_size, block_size);
+  if (blocks == 0) return ESM_GFX950_OK;
+  ESM_REQUIRE(ctx, k && means, "key_block_means: null pointer");
+  ESM_REQUIRE(ctx, ldk >= cols, "key_block_means: ldk must be >= num_kv_heads * head_dim");
+  ESM_REQUIRE(ctx, aligned(k, size) && aligned(means, 4), "key_block_means: misaligned pointer");
+  ESM_REQUIRE(ctx, !bytes_overlap(k, span_bytes(cu_k[batch_size], ldk, cols, size), means, blocks * cols * 4),
+              "key_block_means: means shares memory with k");
+  DeviceScope on(ctx);
+  try {
+    SeqTable t;
+    void* unused = nullptr;
+    ESM_TRY(stage_sequences(ctx, nullptr, cu_k, batch_size, block_size, 0, &t, &unused));
+    BlockAttnArgs p;
+    p.k = k;
+    p.ldkv = ldk;
+    p.heads = p.kv_heads = num_kv_heads;
+    p.head_dim = head_dim;
+    p.block_size = block_size;
+    p.num_blocks = static_cast<int>(blocks);
+    p.means_out = means;
+    ESM_HIP(ctx, launch_block_means(p, t, dtype, ctx->stream));
+  } catch (const std::exception& e) {
+    return ctx->fail(ESM_GFX950_INTERNAL, std::string("key_block_means: ") + e.what());
+  }
+  return ESM_GFX950_OK;
+}
+
+extern "C" int esm_gfx950_attention_select_blocks(esm_gfx950_ctx* ctx, const void* q, int ldq, const float* means,
+                                                  const int* cu_q, const int* cu_k, int batch_size, int num_heads,
+                                                  int num_kv_heads, int head_dim, int block_size, int top, int* blocks,
+                                                  int dtype) {
+  if (!ctx) return ESM_GFX950_INVALID_ARGUMENT;
+  ESM_TRY(validate_batch(ctx, cu_q, batch_size, -1));
+  ESM_TRY(validate_batch(ctx, cu_k, batch_size, -1));
+  ESM_TRY(check_block_shape(ctx, "attention_select_blocks", num_heads, num_kv_heads, head_dim, block_size, dtype));
+  ESM_REQUIRE(ctx, top >= 1 && top <= kMaxTop, "attention_select_blocks: top must be 1..256");
+  const int rows = cu_q[batch_size], cols = num_heads * head_dim, size = elem_size(dtype);
+  if (rows == 0) return ESM_GFX950_OK;
+  const size_t n_blocks = count_blocks(cu_k, batch_size, block_size);
+  ESM_REQUIRE(ctx, q && blocks && (means || n_blocks == 0), "attention_select_blocks: null pointer");
+  ESM_REQUIRE(ctx, ldq >= cols, "attention_select_blocks: ldq must be >= num_heads * head_dim");
+  ESM_REQUIRE(ctx, aligned(q, size) && aligned(means, 4) && aligned(blocks, 4),
+              "attention_select_blocks: misaligned pointer");
+  ESM_REQUIRE(ctx, static_cast<size_t>(rows) * num_heads <= 0x7fffffff, "attention_select_blocks: too many rows");
+  const size_t out_bytes = static_cast<size_t>(rows) * num_heads * top * 4;
+  ESM_REQUIRE(ctx, !bytes_overlap(q, span_bytes(rows, ldq, cols, size), blocks, out_bytes) &&
+                       !bytes_overlap(means, n_blocks * num_kv_heads * head_dim * 4, blocks, out_bytes),
+              "attention_select_blocks: blocks shares memory with an input");
+  DeviceScope on(ctx);
+  try {
+    SeqTable t;
+    void* unused = nullptr;
+    ESM_TRY(stage_sequences(ctx, cu_q, cu_k, batch_size, block_size, 0, &t, &unused));
+    BlockAttnArgs p;
+    p.q = q;
+    p.ldq = ldq;
+    p.rows = rows;
+    p.heads = num_heads;
+    p.kv_heads = num_kv_heads;
+    p.head_dim = head_dim;
+    p.block_size = block_size;
+    p.top = top;
+    p.num_blocks = static_cast<int>(n_blocks);
+    p.means = means;
+    p.blocks_out = blocks;
+    ESM_HIP(ctx, launch_select_blocks(p, t, dtype, ctx->stream));
+  } catch (const std::exception& e) {
+    return ctx->fail(ESM_GFX950_INTERNAL, std::string("attention_select_blocks: ") + e.what());
+  }
+  return ESM_GFX950_OK;
+}
+
+extern "C" int esm_gfx950_attention_blocks(esm_gfx950_ctx* ctx, const void* q, int ldq, const void* k, const void* v,
+                                           int ldkv, const int* blocks, const int* cu_q, const int* cu_k,
+                                           int batch_size, int num_heads, int num_kv_heads, int head_dim,
+                                           int block_size, int top, void* out, int dtype) {
+  if (!ctx) return ESM_GFX950_INVALID_ARGUMENT;
+  ESM_TRY(validate_batch(ctx, cu_q, batch_size, -1));
+  ESM_TRY(validate_batch(ctx, cu_k, batch_size, -1));
+  ESM_TRY(check_block_shape(ctx, "attention_blocks", num_heads, num_kv_heads, head_dim, block_size, dtype));
+  ESM_REQUIRE(ctx, top >= 1 && top <= kMaxTop, "attention_blocks: top must be 1..256");
+  const int rows = cu_q[batch_size], keys = cu_k[batch_size], cols = num_heads * head_dim,
+            kv_cols = num_kv_heads * head_dim, size = elem_size(dtype);
+  if (rows == 0) return ESM_GFX950_OK;
+  ESM_REQUIRE(ctx, q && blocks && out && ((k && v) || keys == 0), "attention_blocks: null pointer");
+  ESM_REQUIRE(ctx, ldq >= cols && ldkv >= kv_cols,
+              "attention_blocks: ldq must be >= num_heads * head_dim and ldkv >= num_kv_heads * head_dim");
+  ESM_REQUIRE(ctx, aligned(q, size) && aligned(k, size) && aligned(v, size) && aligned(out, size) && aligned(blocks, 4),
+              "attention_blocks: misaligned pointer");
+  ESM_REQUIRE(ctx, static_cast<size_t>(rows) * num_heads <= 0x7fffffff, "attention_blocks: too many rows");
+  const size_t out_bytes = static_cast<size_t>(rows) * cols * size, kv_bytes = span_bytes(keys, ldkv, kv_cols, size);
+  ESM_REQUIRE(ctx, !bytes_overlap(q, span_bytes(rows, ldq, cols, size), out, out_bytes) &&
+                       !bytes_overlap(k, kv_bytes, out, out_bytes) && !bytes_overlap(v, kv_bytes, out, out_bytes) &&
+                       !bytes_overlap(blocks, static_cast<size_t>(rows) * num_heads * top * 4, out, out_bytes),
+              "attention_blocks: out shares memory with an input");
+  DeviceScope on(ctx);
+  try {
+    BlockAttnArgs p;
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.ldq = ldq;
+    p.ldkv = ldkv;
+    p.rows = rows;
+    p.heads = num_heads;
+    p.kv_heads = num_kv_heads;
+    p.head_dim = head_dim;
+    p.block_size = block_size;
+    p.top = top;
+    p.num_blocks = static_cast<int>(count_blocks(cu_k, batch_size, block_size));
+    p.blocks = blocks;
+    p.out = out;
+    SeqTable t;
+    void* unused = nullptr;
+    ESM_TRY(stage_sequences(ctx, cu_q, cu_k, batch_size, block_size, 0, &t, &unused));
+    ESM_HIP(ctx, launch_attention_blocks(p, t, dtype, ctx->stream));
+  } catch (const std::exception& e) {
+    return ctx->fail(ESM_GFX950_INTERNAL, std::string("attention_blocks: ") + e.what());
+  }
   return ESM_GFX950_OK;
 }
 

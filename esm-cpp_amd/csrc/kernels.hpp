@@ -335,6 +335,62 @@ hipError_t launch_embed(const int* ids, const float* tok_scale,
 hipError_t launch_cast_f32(const float* x, size_t n, uint16_t* out,
                            int to_bf16, hipStream_t s);
 
+// ------------------------------------------------------------ 4-bit linears
+// Element types of the operators below (values of ESM_GFX950_F32 ...).
+enum ElemType : int { kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 2 };
+
+// C[m, n] = sum_k A[m, k] W[n, k] + bias[n] with 4-bit W in linear_i4_layout's
+// order; A and C of one ElemType, bias fp32 or null.
+struct LinearI4Args {
+  const void* A = nullptr;
+  int lda = 0;
+  const uint32_t* W = nullptr;
+  const float* scales = nullptr;
+  const float* bias = nullptr;
+  void* C = nullptr;
+  int ldc = 0;
+  int M = 0, N = 0, K = 0;
+  int group = 0;    // 32, 64 or a multiple of 128
+  int groups = 0;   // ceil(K / group)
+  int tiles_k = 0;  // ceil(K / 128)
+  bool vec_a = false;  // A's rows start at 16-byte addresses
+};
+hipError_t launch_linear_i4(const LinearI4Args& p, int type, hipStream_t s);
+// The device layout (host): w of 256 dwords per 16 x 128 tile, zero codes past N
+// and K; s [tiles_n, groups, 16], zeros past N.
+void linear_i4_layout(const uint8_t* packed, const float* scales, int N, int K, int group, uint32_t* w, float* s);
+
+// ------------------------------------------------------------ block attention
+// A packed batch's query and key offsets and its key blocks' (sequence b's
+// blocks are cb[b] .. cb[b + 1]), in the kernel's arguments up to kInlineSeqs
+// sequences, so that a call copies nothing; from device memory past that.
+constexpr int kInlineSeqs = 64;
+struct SeqTable {
+  int batch = 0;
+  const int* dev = nullptr;  // cu_q, cu_k, cb one after the other, batch + 1 each
+  int cu_q[kInlineSeqs + 1];
+  int cu_k[kInlineSeqs + 1];
+  int cb[kInlineSeqs + 1];
+};
+struct BlockAttnArgs {
+  const void* q = nullptr;  // [rows, heads, head_dim], row stride ldq
+  const void* k = nullptr;  // [keys, kv_heads, head_dim], row stride ldkv
+  const void* v = nullptr;
+  int ldq = 0, ldkv = 0;
+  int rows = 0, heads = 0, kv_heads = 0, head_dim = 0;
+  int block_size = 0, top = 0;
+  int num_blocks = 0;              // of the batch
+  const float* means = nullptr;    // [num_blocks, kv_heads, head_dim] (select)
+  float* means_out = nullptr;      // (means)
+  const int* blocks = nullptr;     // [rows, heads, top] (attention)
+  int* blocks_out = nullptr;       // (select)
+  void* out = nullptr;             // [rows, heads * head_dim]
+};
+constexpr int kMaxHeadDim = 128, kMaxTop = 256;
+hipError_t launch_block_means(const BlockAttnArgs& p, const SeqTable& t, int type, hipStream_t s);
+hipError_t launch_select_blocks(const BlockAttnArgs& p, const SeqTable& t, int type, hipStream_t s);
+hipError_t launch_attention_blocks(const BlockAttnArgs& p, const SeqTable& t, int type, hipStream_t s);
+
 // ------------------------------------------- the reference's x86 kernels
 // Bit-exact counterparts of the reference's AVX-512 kernels (x86_exact.hip):
 // LayerNormAvx512 (optional residual add before, per-tensor absmax and fp16

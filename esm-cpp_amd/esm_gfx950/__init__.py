@@ -29,6 +29,9 @@ ATTN_MODE_FP16 = 0
 ATTN_MODE_BF16 = 1
 ATTN_MODE_FP32 = 2
 ATTN_MODE_F16X3 = 3
+F32 = 0
+F16 = 1
+BF16 = 2
 NUMERICS_DEFAULT = 0
 NUMERICS_X86_AVX512 = 1
 NUMERICS_X86_AMX = 2
@@ -58,7 +61,9 @@ EXPORTED = [
     "esm_gfx950_attention_varlen_avx512", "esm_gfx950_model_set_numerics", "esm_gfx950_linear_i8_noalloc",
     "esm_gfx950_model_set_ffn_intermediate_bits", "esm_gfx950_linear_i8_gelu_quant_r24",
     "esm_gfx950_forward_hidden_states", "esm_gfx950_forward_packed_masked", "esm_gfx950_batch_upload_masked",
-    "esm_gfx950_model_get_config",
+    "esm_gfx950_model_get_config", "esm_gfx950_weight_upload_i4", "esm_gfx950_weight_free_i4",
+    "esm_gfx950_linear_i4", "esm_gfx950_key_blocks", "esm_gfx950_key_block_means",
+    "esm_gfx950_attention_select_blocks", "esm_gfx950_attention_blocks",
 ]
 
 
@@ -111,6 +116,14 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "esm_gfx950_linear_i8": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32]),
         "esm_gfx950_linear_i8_noalloc": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32]),
         "esm_gfx950_linear_f32": (i32, [vp, vp, vp, vp, vp, i32, i32, i32]),
+        "esm_gfx950_weight_upload_i4": (i32, [vp, vp, vp, i32, i32, i32, C.POINTER(vp)]),
+        "esm_gfx950_weight_free_i4": (i32, [vp, vp]),
+        "esm_gfx950_linear_i4": (i32, [vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32]),
+        "esm_gfx950_key_blocks": (i32, [vp, i32, i32, vp]),
+        "esm_gfx950_key_block_means": (i32, [vp, vp, i32, vp, i32, i32, i32, i32, vp, i32]),
+        "esm_gfx950_attention_select_blocks": (i32, [vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, i32]),
+        "esm_gfx950_attention_blocks": (i32, [vp, vp, i32, vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp,
+                                              i32]),
         "esm_gfx950_layernorm": (i32, [vp, vp, vp, vp, f32, vp, i32, i32]),
         "esm_gfx950_gelu": (i32, [vp, vp, vp, sz]),
         "esm_gfx950_residual_add": (i32, [vp, vp, vp, sz]),
@@ -225,6 +238,16 @@ def attention_work_items(cu: np.ndarray, num_heads: int, mfma: int = True):
     return int(items.value), int(cap.value)
 
 
+def key_blocks(cu_k: np.ndarray, block_size: int) -> np.ndarray:
+    """Offsets [batch + 1] of each sequence's key blocks among the batch's (host only)."""
+    cu_k = np.ascontiguousarray(cu_k, np.int32)
+    out = np.zeros(len(cu_k), np.int32)
+    rc = load_library().esm_gfx950_key_blocks(_ptr(cu_k), len(cu_k) - 1, int(block_size), _ptr(out))
+    if rc != OK:
+        raise Gfx950Error(rc, "key_blocks: invalid arguments")
+    return out
+
+
 def plan_batches(lengths, max_batch_size: int = 256, imbalance_threshold: float = 1.2):
     """PlanBatches on the host: list of groups of caller indices
     (reference src/sched/scheduler.cpp:54-75, defaults of scheduler.h:8-21)."""
@@ -295,6 +318,27 @@ class Weight:
     def free(self):
         if self.handle:
             self.dev.lib.esm_gfx950_weight_free(self.dev.ctx, self.handle)
+            self.handle = None
+
+
+class WeightI4:
+    """A 4-bit weight on the device (esm_gfx950_weight_upload_i4): packed uint8
+    [N, (K + 1) / 2] of codes + 8 (even inputs in the low nibbles), scales fp32
+    [N, ceil(K / group)]."""
+
+    def __init__(self, dev: "Device", packed: np.ndarray, scales: np.ndarray, K: int, group: int):
+        packed = np.ascontiguousarray(packed, np.uint8)
+        scales = np.ascontiguousarray(scales, np.float32)
+        N, K, group = int(packed.shape[0]), int(K), int(group)
+        if packed.shape != (N, (K + 1) // 2) or group <= 0 or scales.shape != (N, (K + group - 1) // group):
+            raise ValueError("packed must be [N, (K + 1) / 2] and scales [N, ceil(K / group)]")
+        h = C.c_void_p()
+        dev._check(dev.lib.esm_gfx950_weight_upload_i4(dev.ctx, _ptr(packed), _ptr(scales), N, K, group, C.byref(h)))
+        self.dev, self.handle, self.N, self.K, self.group = dev, h, N, K, group
+
+    def free(self):
+        if self.handle:
+            self.dev.lib.esm_gfx950_weight_free_i4(self.dev.ctx, self.handle)
             self.handle = None
 
 
@@ -387,6 +431,17 @@ class Device:
                                                           bias.ptr if bias is not None else None, C_out.ptr, M, N, K,
                                                           mode))
 
+    def weight_i4(self, packed: np.ndarray, scales: np.ndarray, K: int, group: int) -> WeightI4:
+        return WeightI4(self, packed, scales, K, group)
+
+    def linear_i4(self, A, W: WeightI4, bias, C_out, M: int, N: int, K: int, dtype: int = F32,
+                  lda: Optional[int] = None, ldc: Optional[int] = None):
+        """C = A W^T + bias with 4-bit weights; A and C of dtype, rows lda / ldc
+        elements apart (default: K / N)."""
+        self._check(self.lib.esm_gfx950_linear_i4(self.ctx, A.ptr, K if lda is None else lda, W.handle,
+                                                  bias.ptr if bias is not None else None, C_out.ptr,
+                                                  N if ldc is None else ldc, M, N, K, dtype))
+
     def linear_f32(self, A, W, bias, C_out, M, N, K):
         self._check(self.lib.esm_gfx950_linear_f32(self.ctx, A.ptr, W.ptr, bias.ptr if bias is not None else None,
                                                    C_out.ptr, M, N, K))
@@ -412,6 +467,35 @@ class Device:
         cu = np.ascontiguousarray(cu, np.int32)
         self._check(self.lib.esm_gfx950_attention_varlen(self.ctx, q.ptr, k.ptr, v.ptr, _ptr(cu), len(cu) - 1, H, dh,
                                                          out.ptr, precision))
+
+    # Block-sparse attention: block means, selection, attention over the selection.
+    def key_block_means(self, k, cu_k: np.ndarray, Hkv: int, dh: int, block_size: int, means, dtype: int = F32,
+                        ldk: Optional[int] = None):
+        """means fp32 [blocks, Hkv, dh] of every key block (key_blocks(cu_k, block_size)[-1] of them)."""
+        cu_k = np.ascontiguousarray(cu_k, np.int32)
+        self._check(self.lib.esm_gfx950_key_block_means(self.ctx, k.ptr, Hkv * dh if ldk is None else ldk, _ptr(cu_k),
+                                                        len(cu_k) - 1, Hkv, dh, block_size, means.ptr, dtype))
+
+    def attention_select_blocks(self, q, means, cu_q: np.ndarray, cu_k: np.ndarray, H: int, Hkv: int, dh: int,
+                                block_size: int, top: int, blocks, dtype: int = F32, ldq: Optional[int] = None):
+        """blocks int32 [queries, H, top]: the blocks whose mean key scores highest, ascending, then -1."""
+        cu_q, cu_k = np.ascontiguousarray(cu_q, np.int32), np.ascontiguousarray(cu_k, np.int32)
+        if len(cu_q) != len(cu_k):
+            raise ValueError("cu_q and cu_k must have the same length")
+        self._check(self.lib.esm_gfx950_attention_select_blocks(
+            self.ctx, q.ptr, H * dh if ldq is None else ldq, means.ptr, _ptr(cu_q), _ptr(cu_k), len(cu_q) - 1, H, Hkv,
+            dh, block_size, top, blocks.ptr, dtype))
+
+    def attention_blocks(self, q, k, v, blocks, cu_q: np.ndarray, cu_k: np.ndarray, H: int, Hkv: int, dh: int,
+                         block_size: int, top: int, out, dtype: int = F32, ldq: Optional[int] = None,
+                         ldkv: Optional[int] = None):
+        """out [queries, H * dh]: attention of every query over its listed blocks alone."""
+        cu_q, cu_k = np.ascontiguousarray(cu_q, np.int32), np.ascontiguousarray(cu_k, np.int32)
+        if len(cu_q) != len(cu_k):
+            raise ValueError("cu_q and cu_k must have the same length")
+        self._check(self.lib.esm_gfx950_attention_blocks(
+            self.ctx, q.ptr, H * dh if ldq is None else ldq, k.ptr, v.ptr, Hkv * dh if ldkv is None else ldkv,
+            blocks.ptr, _ptr(cu_q), _ptr(cu_k), len(cu_q) - 1, H, Hkv, dh, block_size, top, out.ptr, dtype))
 
     # The reference's x86 AVX-512 kernels, bit for bit.
     def layernorm_avx512(self, x, gamma, beta, eps, out, rows, d):

@@ -87,6 +87,29 @@ def quantize_weight(W: np.ndarray) -> Tuple[np.ndarray, np.ndarray]:
     return q, scale
 
 
+def quantize_weight_i4(W: np.ndarray, group: int) -> Tuple[np.ndarray, np.ndarray]:
+    """Symmetric 4-bit codes with one scale per group of inputs, as
+    Device.weight_i4 takes them: (packed uint8 [N, (K + 1) / 2], scales fp32
+    [N, ceil(K / group)]).
+
+    scale = max|W| / 7 of the group (0 where it is all zero), code =
+    clamp(rint(W / scale), -8, 7), stored as code + 8 with even inputs in the
+    low nibbles.
+    """
+    W = np.ascontiguousarray(W, np.float32)
+    N, K = W.shape
+    groups = (K + group - 1) // group
+    wg = np.zeros((N, groups * group), np.float32)
+    wg[:, :K] = W
+    wg = wg.reshape(N, groups, group)
+    scales = (np.max(np.abs(wg), axis=2) / np.float32(7.0)).astype(np.float32)
+    safe = np.where(scales == 0, np.float32(1.0), scales)
+    codes = np.clip(np.rint(wg / safe[:, :, None]), -8, 7).astype(np.int32).reshape(N, -1)[:, :K] + 8
+    if K % 2:
+        codes = np.concatenate([codes, np.full((N, 1), 8, np.int32)], axis=1)
+    return (codes[:, 0::2] | (codes[:, 1::2] << 4)).astype(np.uint8), scales
+
+
 def _smooth_factors(seed: int, name: str, n: int) -> np.ndarray:
     u = _rng(seed, name).uniform(np.log(0.5), np.log(2.0), size=n)
     return np.exp(u).astype(np.float32)

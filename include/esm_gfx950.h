@@ -86,8 +86,13 @@ enum {
  * 218-309; on shapes its gate admits: T >= 32, N % 32 == 0, K % 64 == 0). */
 enum { ESM_GFX950_NUMERICS_DEFAULT = 0, ESM_GFX950_NUMERICS_X86_AVX512 = 1, ESM_GFX950_NUMERICS_X86_AMX = 2 };
 
+/* Element type of the activations of the 4-bit linear and of the block
+ * attention's tensors (inputs and outputs alike). */
+enum { ESM_GFX950_F32 = 0, ESM_GFX950_F16 = 1, ESM_GFX950_BF16 = 2 };
+
 typedef struct esm_gfx950_ctx esm_gfx950_ctx;
 typedef struct esm_gfx950_weight esm_gfx950_weight;
+typedef struct esm_gfx950_weight_i4 esm_gfx950_weight_i4;
 typedef struct esm_gfx950_model esm_gfx950_model;
 typedef struct esm_gfx950_observer esm_gfx950_observer;
 
@@ -233,6 +238,31 @@ int esm_gfx950_linear_i8(esm_gfx950_ctx* ctx, const float* A, const esm_gfx950_w
 int esm_gfx950_linear_i8_noalloc(esm_gfx950_ctx* ctx, const float* A, const esm_gfx950_weight* W,
                                  const float* bias, float* C, int M, int N, int K, int act_mode);
 
+/* ---------------------------------------------------------- 4-bit weights
+ * Linears whose weights take half a byte: no counterpart in the reference,
+ * whose smallest weights are int8. W[n, k] = c[n, k] * scales[n, k / group]
+ * with codes c in -8..7. Half of an INT8 weight's bytes, which is what a call
+ * on one or a few rows (a masked position, one short protein) waits for.
+ *
+ * packed: HOST [N, (K + 1) / 2] bytes, code k of a row in byte k / 2, low
+ * nibble for even k, as c + 8 (the nibble behind an odd K is ignored). scales:
+ * HOST fp32 [N, ceil(K / group)], any finite values. group: 32, 64 or a
+ * multiple of 128; the last group of a row may be short. The codes are laid
+ * out once for the matrix cores: 16 x 128 tiles, N and K padded to them. */
+int esm_gfx950_weight_upload_i4(esm_gfx950_ctx* ctx, const uint8_t* packed, const float* scales, int N, int K,
+                                int group, esm_gfx950_weight_i4** out);
+int esm_gfx950_weight_free_i4(esm_gfx950_ctx* ctx, esm_gfx950_weight_i4* w);
+/* C[m, n] = sum_k A[m, k] W[n, k] + bias[n]: A [M, K] with rows lda elements
+ * apart, C [M, N] with rows ldc elements apart (columns past N are left as they
+ * were), both of `dtype` (ESM_GFX950_F32 / F16 / BF16), DEVICE pointers at any
+ * alignment of their type; bias fp32 [N] or NULL. Activations are not
+ * quantised: products of fp32 ones carry 22 significant bits (relative to a
+ * row's largest of 128 inputs, when that is 2^26 times larger), sums are fp32,
+ * rounded once to dtype. C must not share memory with A. M == 0 is a no-op.
+ * N and K must be the weight's (SHAPE_MISMATCH). */
+int esm_gfx950_linear_i4(esm_gfx950_ctx* ctx, const void* A, int lda, const esm_gfx950_weight_i4* W,
+                         const float* bias, void* C, int ldc, int M, int N, int K, int dtype);
+
 /* ----------------------------------------------------------- FP32 / misc ops
  * esm::kernels::Linear (kernels.h:19-20; LinearRef gemm_fp32.cpp:33-46):
  * C[M, N] = A[M, K] W[N, K]^T + bias (bias may be NULL). */
@@ -290,6 +320,50 @@ int esm_gfx950_attention_varlen(esm_gfx950_ctx* ctx, const float* q, const float
 int esm_gfx950_attention_varlen_bf16(esm_gfx950_ctx* ctx, const uint16_t* q, const uint16_t* k,
                                      const uint16_t* v, int v_is_fp16, const int* cu_seqlens,
                                      int batch_size, int num_heads, float* out);
+
+/* ------------------------------------------------- block-sparse attention
+ * Attention of every query over a few blocks of keys, for sequences so long
+ * that esm_gfx950_attention_varlen's L^2 is what a forward waits for, and for a
+ * few query positions against a long sequence. No counterpart in the reference.
+ * Three calls: the mean key of every block; for every query and head the `top`
+ * blocks whose mean has the largest product with the query; the attention over
+ * those blocks alone.
+ *
+ * Sequence b has queries cu_q[b] .. cu_q[b + 1] and keys cu_k[b] ..
+ * cu_k[b + 1] (HOST arrays of batch_size + 1, as cu_seqlens; the same array
+ * for self-attention). Its keys form ceil(keys / block_size) blocks, the last
+ * one perhaps short; the batch's blocks follow one another in sequence order.
+ * block_size: a multiple of 16, 16..1024. q [cu_q.back(), num_heads, head_dim]
+ * (pre-scaled, as esm_gfx950_attention_varlen's) with rows ldq elements apart,
+ * k and v [cu_k.back(), num_kv_heads, head_dim] with rows ldk elements apart:
+ * DEVICE memory of dtype (ESM_GFX950_F32 / F16 / BF16), so Q, K and V may be
+ * parts of one fused row. Query head h reads key head h / (num_heads /
+ * num_kv_heads); num_kv_heads divides num_heads. head_dim: a multiple of 8, at
+ * most 128. */
+/* Host only: the block offsets [batch_size + 1] of a batch. */
+int esm_gfx950_key_blocks(const int* cu_k, int batch_size, int block_size, int* cu_blocks);
+/* means fp32 [blocks, num_kv_heads, head_dim]: every block's mean key, summed in
+ * 64 bits. Needed once per set of keys, however many queries follow. */
+int esm_gfx950_key_block_means(esm_gfx950_ctx* ctx, const void* k, int ldk, const int* cu_k, int batch_size,
+                               int num_kv_heads, int head_dim, int block_size, float* means, int dtype);
+/* blocks int32 [cu_q.back(), num_heads, top], 1 <= top <= 256: the indices
+ * (within the query's sequence) of its highest-scoring blocks, ascending, then
+ * -1 where the sequence has fewer. Scores order as in 64 bits; equal ones go to
+ * the lowest index, and a NaN counts as -inf. */
+int esm_gfx950_attention_select_blocks(esm_gfx950_ctx* ctx, const void* q, int ldq, const float* means,
+                                       const int* cu_q, const int* cu_k, int batch_size, int num_heads,
+                                       int num_kv_heads, int head_dim, int block_size, int top, int* blocks,
+                                       int dtype);
+/* out [cu_q.back(), num_heads * head_dim] of dtype: softmax over the keys of
+ * the row's listed blocks, times v; fp32 softmax and sums, operands of fp32
+ * tensors carried to 22 significant bits. blocks as above, in any order, the
+ * caller's own choice or attention_select_blocks': an entry that is negative,
+ * past the sequence's blocks or a repeat of an earlier one of its row counts
+ * for nothing, and a row without entries (or keys) is zero. out must not share
+ * memory with q, k, v or blocks. */
+int esm_gfx950_attention_blocks(esm_gfx950_ctx* ctx, const void* q, int ldq, const void* k, const void* v, int ldkv,
+                                const int* blocks, const int* cu_q, const int* cu_k, int batch_size, int num_heads,
+                                int num_kv_heads, int head_dim, int block_size, int top, void* out, int dtype);
 
 /* ----------------------------------------------- the reference's x86 kernels
  * Device counterparts of the AVX-512 arms of the reference's facade, equal
