@@ -1001,6 +1001,9 @@ extern "C" int esm_gfx950_linear_i4(esm_gfx950_ctx* ctx, const void* A, int lda,
 
 // ------------------------------------------------------------ block attention
 namespace {
+// Largest row stride, in elements: a block's 1024 rows stay within 32-bit offsets.
+constexpr int kMaxRowStride = 1 << 22;
+
 // Blocks of n keys.
 int blocks_of(int n, int block_size) { return n > 0 ? (n - 1) / block_size + 1 : 0; }
 
@@ -1092,7 +1095,8 @@ extern "C" int esm_gfx950_key_block_means(esm_gfx950_ctx* ctx, const void* k, in
   const size_t blocks = count_blocks(cu_k, batch_size, block_size);
   if (blocks == 0) return ESM_GFX950_OK;
   ESM_REQUIRE(ctx, k && means, "key_block_means: null pointer");
-  ESM_REQUIRE(ctx, ldk >= cols, "key_block_means: ldk must be >= num_kv_heads * head_dim");
+  ESM_REQUIRE(ctx, ldk >= cols && ldk <= kMaxRowStride,
+              "key_block_means: ldk must be >= num_kv_heads * head_dim, at most 2^22");
   ESM_REQUIRE(ctx, aligned(k, size) && aligned(means, 4), "key_block_means: misaligned pointer");
   ESM_REQUIRE(ctx, !bytes_overlap(k, span_bytes(cu_k[batch_size], ldk, cols, size), means, blocks * cols * 4),
               "key_block_means: means shares memory with k");
@@ -1129,7 +1133,8 @@ extern "C" int esm_gfx950_attention_select_blocks(esm_gfx950_ctx* ctx, const voi
   if (rows == 0) return ESM_GFX950_OK;
   const size_t n_blocks = count_blocks(cu_k, batch_size, block_size);
   ESM_REQUIRE(ctx, q && blocks && (means || n_blocks == 0), "attention_select_blocks: null pointer");
-  ESM_REQUIRE(ctx, ldq >= cols, "attention_select_blocks: ldq must be >= num_heads * head_dim");
+  ESM_REQUIRE(ctx, ldq >= cols && ldq <= kMaxRowStride,
+              "attention_select_blocks: ldq must be >= num_heads * head_dim, at most 2^22");
   ESM_REQUIRE(ctx, aligned(q, size) && aligned(means, 4) && aligned(blocks, 4),
               "attention_select_blocks: misaligned pointer");
   ESM_REQUIRE(ctx, static_cast<size_t>(rows) * num_heads <= 0x7fffffff, "attention_select_blocks: too many rows");
@@ -1174,8 +1179,8 @@ extern "C" int esm_gfx950_attention_blocks(esm_gfx950_ctx* ctx, const void* q, i
             kv_cols = num_kv_heads * head_dim, size = elem_size(dtype);
   if (rows == 0) return ESM_GFX950_OK;
   ESM_REQUIRE(ctx, q && blocks && out && ((k && v) || keys == 0), "attention_blocks: null pointer");
-  ESM_REQUIRE(ctx, ldq >= cols && ldkv >= kv_cols,
-              "attention_blocks: ldq must be >= num_heads * head_dim and ldkv >= num_kv_heads * head_dim");
+  ESM_REQUIRE(ctx, ldq >= cols && ldkv >= kv_cols && ldq <= kMaxRowStride && ldkv <= kMaxRowStride,
+              "attention_blocks: ldq must be >= num_heads * head_dim and ldkv >= num_kv_heads * head_dim, at most 2^22");
   ESM_REQUIRE(ctx, aligned(q, size) && aligned(k, size) && aligned(v, size) && aligned(out, size) && aligned(blocks, 4),
               "attention_blocks: misaligned pointer");
   ESM_REQUIRE(ctx, static_cast<size_t>(rows) * num_heads <= 0x7fffffff, "attention_blocks: too many rows");
@@ -1201,10 +1206,13 @@ extern "C" int esm_gfx950_attention_blocks(esm_gfx950_ctx* ctx, const void* q, i
     p.num_blocks = static_cast<int>(count_blocks(cu_k, batch_size, block_size));
     p.blocks = blocks;
     p.out = out;
+    p.vec_q = aligned(q, 16) && static_cast<size_t>(ldq) * size % 16 == 0;
+    p.vec_kv = aligned(k, 16) && aligned(v, 16) && static_cast<size_t>(ldkv) * size % 16 == 0;
+    const BlockAttnPlan plan = attention_blocks_plan(p);
     SeqTable t;
-    void* unused = nullptr;
-    ESM_TRY(stage_sequences(ctx, cu_q, cu_k, batch_size, block_size, 0, &t, &unused));
-    ESM_HIP(ctx, launch_attention_blocks(p, t, dtype, ctx->stream));
+    void* scratch = nullptr;
+    ESM_TRY(stage_sequences(ctx, cu_q, cu_k, batch_size, block_size, plan.scratch_bytes, &t, &scratch));
+    ESM_HIP(ctx, launch_attention_blocks(p, t, plan, scratch, dtype, ctx->stream));
   } catch (const std::exception& e) {
     return ctx->fail(ESM_GFX950_INTERNAL, std::string("attention_blocks: ") + e.what());
   }

@@ -385,11 +385,21 @@ struct BlockAttnArgs {
   const int* blocks = nullptr;     // [rows, heads, top] (attention)
   int* blocks_out = nullptr;       // (select)
   void* out = nullptr;             // [rows, heads * head_dim]
+  bool vec_q = false, vec_kv = false;  // heads start at 16-byte addresses
 };
 constexpr int kMaxHeadDim = 128, kMaxTop = 256;
 hipError_t launch_block_means(const BlockAttnArgs& p, const SeqTable& t, int type, hipStream_t s);
 hipError_t launch_select_blocks(const BlockAttnArgs& p, const SeqTable& t, int type, hipStream_t s);
-hipError_t launch_attention_blocks(const BlockAttnArgs& p, const SeqTable& t, int type, hipStream_t s);
+// How attention_blocks runs: row by row, or block by block (grouped) for
+// `tokens` tokens and `kv_heads` key heads at a time.
+struct BlockAttnPlan {
+  bool grouped = false;
+  int tokens = 0, kv_heads = 0;
+  size_t scratch_bytes = 0;
+};
+BlockAttnPlan attention_blocks_plan(const BlockAttnArgs& p);
+hipError_t launch_attention_blocks(const BlockAttnArgs& p, const SeqTable& t, const BlockAttnPlan& plan, void* scratch,
+                                   int type, hipStream_t s);
 
 // ------------------------------------------- the reference's x86 kernels
 // Bit-exact counterparts of the reference's AVX-512 kernels (x86_exact.hip):

@@ -337,7 +337,7 @@ int esm_gfx950_attention_varlen_bf16(esm_gfx950_ctx* ctx, const uint16_t* q, con
  * (pre-scaled, as esm_gfx950_attention_varlen's) with rows ldq elements apart,
  * k and v [cu_k.back(), num_kv_heads, head_dim] with rows ldk elements apart:
  * DEVICE memory of dtype (ESM_GFX950_F32 / F16 / BF16), so Q, K and V may be
- * parts of one fused row. Query head h reads key head h / (num_heads /
+ * parts of one fused row (row strides are at most 2^22). Query head h reads key head h / (num_heads /
  * num_kv_heads); num_kv_heads divides num_heads. head_dim: a multiple of 8, at
  * most 128. */
 /* Host only: the block offsets [batch_size + 1] of a batch. */
@@ -359,7 +359,11 @@ int esm_gfx950_attention_select_blocks(esm_gfx950_ctx* ctx, const void* q, int l
  * tensors carried to 22 significant bits. blocks as above, in any order, the
  * caller's own choice or attention_select_blocks': an entry that is negative,
  * past the sequence's blocks or a repeat of an earlier one of its row counts
- * for nothing, and a row without entries (or keys) is zero. out must not share
+ * for nothing, and a row without entries (or keys) is zero. Results do not
+ * depend on what runs beside a call, nor on the order of entries beyond
+ * rounding. A row may be NaN where its query, or a key or value of a block that
+ * it lists, holds an infinity or a NaN. Scratch that grows with
+ * cu_q.back() * num_heads * top stays with the context. out must not share
  * memory with q, k, v or blocks. */
 int esm_gfx950_attention_blocks(esm_gfx950_ctx* ctx, const void* q, int ldq, const void* k, const void* v, int ldkv,
                                 const int* blocks, const int* cu_q, const int* cu_k, int batch_size, int num_heads,
