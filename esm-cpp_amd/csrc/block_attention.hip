@@ -21,15 +21,17 @@ namespace {
 // Parts of the grouped attention that are in flight between the pass that
 // writes them and the one that joins them: what the 256 MB memory-side cache
 // holds beside the keys.
-constexpr size_t kPartBytes = size_t{128} << 20;
+constexpr size_t kPartBytes = size_t{160} << 20;
 
 // The grouped attention's device scratch (attention, block by block).
 struct GroupedWork {
   int token0 = 0, tokens = 0;  // the tokens in hand
+  int head_entries = 0;        // entries of a key head, counting or not
+  int head_tiles = 0;          // most tiles of a key head
   int* counts = nullptr;       // [cells] entries
+  int* used = nullptr;         // [kv_heads] tiles of a key head
   int* first = nullptr;        // [cells] first entry in list
-  int* cell_tile = nullptr;    // [cells + 1] first tile
-  int4* tiles = nullptr;       // (cell, first entry, entries, -)
+  int4* tiles = nullptr;       // [kv_heads, head_tiles] (cell, first entry, entries, -)
   int* place = nullptr;        // [entries] place in its cell, -1: does not count
   int* list = nullptr;         // [entries] by cell
   float2* part_ml = nullptr;   // [entries of the heads in hand] maximum (base 2) and sum
@@ -177,16 +179,17 @@ __device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) {
 }
 
 // The exponent e for which amax * 2^e lies in [2^14, 2^15), where fp16 holds
-// hi + lo parts to 22 bits and everything 2^-39 above the largest.
+// hi + lo parts to 22 bits down to 2^-39 of the largest; within -60 .. 60, so
+// that the inverse of a product of two such scales is a normal number.
 __device__ __forceinline__ int scale_exponent(float amax) {
-  return amax > 0.0f ? max(-120, min(120, 15 - __builtin_amdgcn_frexp_expf(amax))) : 0;
+  return amax > 0.0f ? max(-60, min(60, 15 - __builtin_amdgcn_frexp_expf(amax))) : 0;
 }
 
 // Eight consecutive elements as fp32.
-template <class T>
-__device__ __forceinline__ void load8(const T* x, bool vec, float (&out)[8]) {
+template <bool VEC, class T>
+__device__ __forceinline__ void load8(const T* x, float (&out)[8]) {
   T v[8];
-  if (vec) {
+  if constexpr (VEC) {
     uint4 p[sizeof(T) / 2];
 #pragma unroll
     for (unsigned i = 0; i < sizeof(T) / 2; ++i) p[i] = reinterpret_cast<const uint4*>(x)[i];
@@ -239,16 +242,6 @@ __device__ __forceinline__ float group_sum(float v) {
   return b.a + b.b;
 }
 
-// Whether entry e of a row's list counts: a block of the sequence, and no
-// repeat of an earlier entry.
-__device__ __forceinline__ bool entry_counts(const int* list, int e, int nb) {
-  const int j = list[e];
-  if (j < 0 || j >= nb) return false;
-  for (int i = 0; i < e; ++i)
-    if (list[i] == j) return false;
-  return true;
-}
-
 }  // namespace
 
 // ------------------------------------------------- attention, row by row
@@ -256,7 +249,7 @@ __device__ __forceinline__ bool entry_counts(const int* list, int e, int nb) {
 // LDS. The 16-byte pieces of a key lie in LPK neighbouring lanes, 64 / LPK keys
 // to a load. After the loads' products a butterfly over the lanes (each step
 // hands half of the lane's values over) leaves every lane one key's score.
-template <int DT, int DH>
+template <int DT, int DH, bool VEC>
 __global__ __launch_bounds__(512) void attention_rows_kernel(BlockAttnArgs p, SeqTable t) {
   using T = typename ElemOf<DT>::T;
   constexpr int DPL = 16 / sizeof(T);        // dims per lane
@@ -296,7 +289,7 @@ __global__ __launch_bounds__(512) void attention_rows_kernel(BlockAttnArgs p, Se
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
           const uint32_t off = static_cast<uint32_t>(min(i * KPI + kl, n - 1)) * static_cast<uint32_t>(p.ldkv) + dl;
-          if (p.vec_kv) {
+          if constexpr (VEC) {
             x[i] = *reinterpret_cast<const uint4*>(at + off);
           } else {
             T y[DPL];
@@ -390,107 +383,140 @@ __global__ __launch_bounds__(512) void attention_rows_kernel(BlockAttnArgs p, Se
 //
 // An entry is (token - token0, head, list index) as one number; cells are
 // numbered key head first.
-constexpr int kCountThreads = 256, kCountEntries = 4096, kCountBlocks = 8192;
-constexpr int kTileEntries = 128;
+constexpr int kCountThreads = 256, kCountPer = 16, kCountEntries = kCountThreads * kCountPer, kCountBlocks = 8192;
+constexpr int kTileEntries = 512;
+
+// The entries of one workgroup of the two list kernels: one head, and as many
+// tokens as give kCountEntries entries (one token where it has more).
+struct EntryRange {
+  int head, hk, first, entries;
+};
+__device__ __forceinline__ EntryRange entry_range(const BlockAttnArgs& p, const GroupedWork& g) {
+  const int per = kCountEntries / p.top, head = blockIdx.x % p.heads, first = blockIdx.x / p.heads * per;
+  return EntryRange{head, head / (p.heads / p.kv_heads), first, min(per, g.tokens - first) * p.top};
+}
 
 // Counts the entries of each cell and gives each entry its place in it (-1: it
-// does not count). One workgroup per head and as many tokens as give
-// kCountEntries entries; their counts meet in LDS first where the batch's blocks
-// fit it, so that a cell sees one atomic per workgroup.
-__global__ __launch_bounds__(kCountThreads) void count_entries_kernel(BlockAttnArgs p, SeqTable t, GroupedWork g,
-                                                                      int tokens_per_group) {
+// does not count). A workgroup's counts meet in LDS first where the batch's
+// blocks fit it, so that a cell sees one atomic per workgroup.
+__global__ __launch_bounds__(kCountThreads) void count_entries_kernel(BlockAttnArgs p, SeqTable t, GroupedWork g) {
   __shared__ int hist[kCountBlocks];
-  const int head = blockIdx.x % p.heads, first = blockIdx.x / p.heads * tokens_per_group;
-  const int tokens = min(tokens_per_group, g.tokens - first);
-  const int hk = head / (p.heads / p.kv_heads);
-  int* cells = g.counts + static_cast<size_t>(hk) * p.num_blocks;
+  __shared__ int unsorted[kCountEntries];  // by token of the range
+  const EntryRange r = entry_range(p, g);
+  int* cells = g.counts + static_cast<size_t>(r.hk) * p.num_blocks;
   const bool lds = p.num_blocks <= kCountBlocks;
+  for (int i = threadIdx.x; lds && i < p.num_blocks; i += kCountThreads) hist[i] = 0;
+  for (int i = threadIdx.x; i < r.entries / p.top; i += kCountThreads) unsorted[i] = 0;
+  __syncthreads();
+  // A list that ascends and then ends in negatives, as the selection's do, has
+  // no repeats.
+  int block[kCountPer], place[kCountPer];
+#pragma unroll
+  for (int u = 0; u < kCountPer; ++u) {
+    const int i = u * kCountThreads + threadIdx.x, tok = i / p.top, e = i - tok * p.top;
+    block[u] = -1;
+    if (i >= r.entries) continue;
+    const int* list = p.blocks + (static_cast<size_t>(g.token0 + r.first + tok) * p.heads + r.head) * p.top;
+    const int j = list[e];
+    if (e > 0 && j >= 0 && (list[e - 1] < 0 || j <= list[e - 1])) unsorted[tok] = 1;
+    block[u] = j;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kCountPer; ++u) {
+    const int i = u * kCountThreads + threadIdx.x, tok = i / p.top, e = i - tok * p.top;
+    place[u] = -1;
+    if (block[u] < 0) continue;
+    const Seq s = seq_at(t, seq_of(t, t.cu_q, 0, g.token0 + r.first + tok));
+    bool counts = block[u] < s.b1 - s.b0;
+    if (unsorted[tok]) {
+      const int* list = p.blocks + (static_cast<size_t>(g.token0 + r.first + tok) * p.heads + r.head) * p.top;
+      for (int k = 0; k < e; ++k) counts &= list[k] != block[u];
+    }
+    if (!counts) continue;
+    block[u] += s.b0;
+    place[u] = atomicAdd(lds ? &hist[block[u]] : &cells[block[u]], 1);
+  }
   if (lds) {
-    for (int i = threadIdx.x; i < p.num_blocks; i += kCountThreads) hist[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.num_blocks; i += kCountThreads) {
+      const int n = hist[i];
+      if (n) hist[i] = atomicAdd(&cells[i], n);
+    }
     __syncthreads();
   }
-  const int entries = tokens * p.top;
-  for (int i = threadIdx.x; i < entries; i += kCountThreads) {
-    const int tok = first + i / p.top, e = i % p.top;
-    const Seq s = seq_at(t, seq_of(t, t.cu_q, 0, g.token0 + tok));
-    const int* list = p.blocks + (static_cast<size_t>(g.token0 + tok) * p.heads + head) * p.top;
-    int place = -1;
-    if (entry_counts(list, e, s.b1 - s.b0)) {
-      const int j = s.b0 + list[e];
-      place = lds ? atomicAdd(&hist[j], 1) : atomicAdd(&cells[j], 1);
+#pragma unroll
+  for (int u = 0; u < kCountPer; ++u) {
+    const int i = u * kCountThreads + threadIdx.x, tok = i / p.top, e = i - tok * p.top;
+    if (i >= r.entries) continue;
+    if (lds && place[u] >= 0) place[u] += hist[block[u]];
+    g.place[(static_cast<size_t>(r.first + tok) * p.heads + r.head) * p.top + e] = place[u];
+  }
+}
+
+// One workgroup per key head: running sums over its cells' entries and tiles give
+// every cell its stretch of the list and its tiles. (One thread per cell with
+// atomics on the head's two totals took 29 us for 129 blocks of 20 heads.)
+constexpr int kPlaceThreads = 512;
+__global__ __launch_bounds__(kPlaceThreads) void place_cells_kernel(BlockAttnArgs p, GroupedWork g) {
+  __shared__ int sums[2][kPlaceThreads / 64];
+  const int hk = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int at0 = hk * g.head_entries, tile0 = hk * g.head_tiles;
+  for (int c0 = 0; c0 < p.num_blocks; c0 += kPlaceThreads) {
+    const int block = c0 + threadIdx.x, c = hk * p.num_blocks + block;
+    const int n = block < p.num_blocks ? g.counts[c] : 0, tiles = (n + kTileEntries - 1) / kTileEntries;
+    int n_to = n, tiles_to = tiles;  // sums over the wave's lanes up to this one
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int a = __shfl_up(n_to, d), b = __shfl_up(tiles_to, d);
+      n_to += lane >= d ? a : 0;
+      tiles_to += lane >= d ? b : 0;
     }
-    g.place[(static_cast<size_t>(tok) * p.heads + head) * p.top + e] = place;
+    if (lane == 63) {
+      sums[0][wave] = n_to;
+      sums[1][wave] = tiles_to;
+    }
+    __syncthreads();
+    int at = at0 + n_to - n, tile = tile0 + tiles_to - tiles;
+#pragma unroll
+    for (int w = 0; w < kPlaceThreads / 64; ++w) {
+      at += w < wave ? sums[0][w] : 0;
+      tile += w < wave ? sums[1][w] : 0;
+      at0 += sums[0][w];
+      tile0 += sums[1][w];
+    }
+    if (n) g.first[c] = at;
+    for (int i = 0; i < tiles; ++i)
+      g.tiles[tile + i] = make_int4(c, at + i * kTileEntries, min(kTileEntries, n - i * kTileEntries), 0);
+    __syncthreads();
   }
-  if (!lds) return;
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.num_blocks; i += kCountThreads) {
-    const int n = hist[i];
-    if (n) hist[i] = atomicAdd(&cells[i], n);
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < entries; i += kCountThreads) {
-    const int tok = first + i / p.top, e = i % p.top;
-    const size_t at = (static_cast<size_t>(tok) * p.heads + head) * p.top + e;
+  if (threadIdx.x == 0) g.used[hk] = tile0 - hk * g.head_tiles;
+}
+
+__global__ __launch_bounds__(kCountThreads) void scatter_entries_kernel(BlockAttnArgs p, SeqTable t, GroupedWork g) {
+  const EntryRange r = entry_range(p, g);
+#pragma unroll
+  for (int u = 0; u < kCountPer; ++u) {
+    const int i = u * kCountThreads + threadIdx.x, tok = i / p.top, e = i - tok * p.top;
+    if (i >= r.entries) continue;
+    const size_t at = (static_cast<size_t>(r.first + tok) * p.heads + r.head) * p.top + e;
     const int place = g.place[at];
     if (place < 0) continue;
-    const Seq s = seq_at(t, seq_of(t, t.cu_q, 0, g.token0 + tok));
-    const int j = s.b0 + p.blocks[(static_cast<size_t>(g.token0 + tok) * p.heads + head) * p.top + e];
-    g.place[at] = place + hist[j];
+    const int j = seq_at(t, seq_of(t, t.cu_q, 0, g.token0 + r.first + tok)).b0 +
+                  p.blocks[static_cast<size_t>(g.token0) * p.heads * p.top + at];
+    g.list[g.first[r.hk * p.num_blocks + j] + place] = static_cast<int>(at);
   }
 }
 
-// One workgroup: the cells' first entries and tiles (running sums over the
-// counts), and the tiles themselves.
-constexpr int kScanThreads = 1024;
-__global__ __launch_bounds__(kScanThreads) void scan_cells_kernel(GroupedWork g, int cells) {
-  __shared__ int sums[2][kScanThreads];
-  const int per = (cells + kScanThreads - 1) / kScanThreads;
-  const int c0 = min(cells, static_cast<int>(threadIdx.x) * per), c1 = min(cells, c0 + per);
-  int entries = 0, tiles = 0;
-  for (int c = c0; c < c1; ++c) {
-    entries += g.counts[c];
-    tiles += (g.counts[c] + kTileEntries - 1) / kTileEntries;
-  }
-  sums[0][threadIdx.x] = entries;
-  sums[1][threadIdx.x] = tiles;
-  __syncthreads();
-  for (int d = 1; d < kScanThreads; d *= 2) {
-    const int a = threadIdx.x >= d ? sums[0][threadIdx.x - d] : 0, b = threadIdx.x >= d ? sums[1][threadIdx.x - d] : 0;
-    __syncthreads();
-    sums[0][threadIdx.x] += a;
-    sums[1][threadIdx.x] += b;
-    __syncthreads();
-  }
-  int at = sums[0][threadIdx.x] - entries, tile = sums[1][threadIdx.x] - tiles;
-  for (int c = c0; c < c1; ++c) {
-    const int n = g.counts[c];
-    g.first[c] = at;
-    g.cell_tile[c] = tile;
-    for (int i = 0; i < n; i += kTileEntries) g.tiles[tile++] = make_int4(c, at + i, min(kTileEntries, n - i), 0);
-    at += n;
-  }
-  if (threadIdx.x == kScanThreads - 1) g.cell_tile[cells] = tile;
-}
-
-__global__ __launch_bounds__(256) void scatter_entries_kernel(BlockAttnArgs p, SeqTable t, GroupedWork g) {
-  const size_t n = static_cast<size_t>(g.tokens) * p.heads * p.top;
-  for (size_t i = blockIdx.x * size_t{256} + threadIdx.x; i < n; i += size_t{256} * gridDim.x) {
-    const int place = g.place[i];
-    if (place < 0) continue;
-    const int row = static_cast<int>(i / p.top), tok = row / p.heads, hk = row % p.heads / (p.heads / p.kv_heads);
-    const Seq s = seq_at(t, seq_of(t, t.cu_q, 0, g.token0 + tok));
-    const int j = s.b0 + p.blocks[static_cast<size_t>(g.token0) * p.heads * p.top + i];
-    g.list[g.first[hk * p.num_blocks + j] + place] = static_cast<int>(i);
-  }
-}
-
-// One workgroup per tile of 128 entries, 32 to a wave. Keys and values come 64
-// at a time through LDS as fp16 (hi and lo planes for fp32 tensors), multiplied
-// by powers of two that bring each 64 x dim tile's largest to [2^14, 2^15), and
-// a row of q likewise: full precision at every magnitude. S^T = K Q^T leaves a
-// lane the scores of one query with keys 4 lg .. + 4 of every 16, which is the
-// operand of O^T = V^T P^T as it stands.
-template <int DT, int DH>
+// One workgroup per tile of up to 512 entries of a cell, 32 at a time to a wave.
+// Keys and values come 64 at a time through LDS as fp16 (hi and lo planes for
+// fp32 tensors), multiplied by powers of two that bring each 64 x dim tile's
+// largest to [2^14, 2^15), and a row of q likewise: full precision at every
+// magnitude. Blocks of at most 64 keys are staged once, and the waves then walk
+// the tile's entries on their own, the next ones' queries on their way. S^T =
+// K Q^T leaves a lane the scores of one query with keys 4 lg .. + 4 of every 16,
+// which is the operand of O^T = V^T P^T as it stands.
+template <int DT, int DH, bool VEC>
 __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, SeqTable t, GroupedWork g, int hk0,
                                                               int hk1) {
   using T = typename ElemOf<DT>::T;
@@ -498,66 +524,26 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
   constexpr int kPitch = DH * 2 + 16;  // 16 rows of 16 bytes fall on distinct banks
   constexpr int kPlane = 64 * kPitch;
   constexpr int kUnits = 64 * DH / 8 / 256;  // 8-element pieces per thread, of K and of V
+  constexpr int KS = DH / 32;
   __shared__ __align__(16) uint8_t tile_k[PL * kPlane], tile_v[PL * kPlane];
   __shared__ float tile_max[2][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int lr = lane & 15, lg = lane >> 4;
-  const int tile0 = g.cell_tile[hk0 * p.num_blocks], tile_end = g.cell_tile[hk1 * p.num_blocks];
-  if (tile0 + static_cast<int>(blockIdx.x) >= tile_end) return;
-  const int4 tile = g.tiles[tile0 + blockIdx.x];
-  const int hk = tile.x / p.num_blocks, block = tile.x % p.num_blocks, dim = p.head_dim;
+  // Workgroup i runs on XCD i % 8, and each XCD has its own L2: the hk1 - hk0 (1,
+  // 2, 4 or 8) key heads in hand get as many XCDs each, whose L2s then hold that
+  // head's queries.
+  const int xcds = 8 / (hk1 - hk0), xcd = blockIdx.x % 8;
+  const int hk = hk0 + xcd / xcds, nth = blockIdx.x / 8 * xcds + xcd % xcds;
+  if (nth >= g.used[hk]) return;
+  const int4 tile = g.tiles[hk * g.head_tiles + nth];
+  const int block = tile.x - hk * p.num_blocks, dim = p.head_dim;
   const Seq s = seq_at(t, seq_of(t, t.cb, 2, block));
   const int key0 = s.k0 + (block - s.b0) * p.block_size, keys = min(p.block_size, s.k1 - key0);
   const int each = p.heads / p.kv_heads, chunk_heads = (hk1 - hk0) * each;
 
-  // This lane's queries.
-  int entry[2], head[2], tok[2];
-  f16x8 qf[2][DH / 32][PL];
-  int qe[2];
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int i = wave * 32 + r * 16 + lr;
-    entry[r] = i < tile.z ? g.list[tile.y + i] : -1;
-  }
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = max(entry[r], 0) / p.top;
-    tok[r] = row / p.heads;
-    head[r] = row % p.heads;
-    const T* q = static_cast<const T*>(p.q) + static_cast<size_t>(g.token0 + tok[r]) * p.ldq + head[r] * dim;
-    float x[DH / 32][8];
-    float amax = 0.0f;
-#pragma unroll
-    for (int ks = 0; ks < DH / 32; ++ks) {
-      const int d = ks * 32 + lg * 8;
-      if (entry[r] >= 0 && d < dim) {
-        load8<T>(q + d, p.vec_q, x[ks]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[ks][i] = 0.0f;
-      }
-      amax = fmaxf(amax, max8(x[ks]));
-    }
-    qe[r] = scale_exponent(group_max(amax));
-    const float mul = __builtin_amdgcn_ldexpf(1.0f, qe[r]);
-#pragma unroll
-    for (int ks = 0; ks < DH / 32; ++ks) {
-      uint4 w[PL];
-      split8<PL>(x[ks], mul, w);
-#pragma unroll
-      for (int pl = 0; pl < PL; ++pl) qf[r][ks][pl] = __builtin_bit_cast(f16x8, w[pl]);
-    }
-  }
-  const bool active = wave * 32 < tile.z;
-
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-  f32x4 o[2][DH / 16];
-#pragma unroll
-  for (int r = 0; r < 2; ++r)
-#pragma unroll
-    for (int db = 0; db < DH / 16; ++db) o[r][db] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  for (int c = 0; c < keys; c += 64) {
+  // Loads the 64 keys from key0 + c on, and their values, into LDS.
+  int ke = 0, ve = 0;
+  auto stage = [&](int c) {
     const int n = min(64, keys - c);
     float kx[kUnits][8], vx[kUnits][8];
     float kmax = 0.0f, vmax = 0.0f;
@@ -566,8 +552,8 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
       const int unit = u * 256 + threadIdx.x, key = unit / (DH / 8), d = unit % (DH / 8) * 8;
       const size_t at = static_cast<size_t>(key0 + c + key) * p.ldkv + hk * dim + d;
       if (key < n && d < dim) {
-        load8<T>(static_cast<const T*>(p.k) + at, p.vec_kv, kx[u]);
-        load8<T>(static_cast<const T*>(p.v) + at, p.vec_kv, vx[u]);
+        load8<VEC>(static_cast<const T*>(p.k) + at, kx[u]);
+        load8<VEC>(static_cast<const T*>(p.v) + at, vx[u]);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) kx[u][i] = vx[u][i] = 0.0f;
@@ -584,9 +570,9 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
       tile_max[0][wave] = kmax;
       tile_max[1][wave] = vmax;
     }
-    __syncthreads();  // also: the last tile's reads are done
-    const int ke = scale_exponent(fmaxf(fmaxf(tile_max[0][0], tile_max[0][1]), fmaxf(tile_max[0][2], tile_max[0][3])));
-    const int ve = scale_exponent(fmaxf(fmaxf(tile_max[1][0], tile_max[1][1]), fmaxf(tile_max[1][2], tile_max[1][3])));
+    __syncthreads();  // also: the last 64 keys' reads are done
+    ke = scale_exponent(fmaxf(fmaxf(tile_max[0][0], tile_max[0][1]), fmaxf(tile_max[0][2], tile_max[0][3])));
+    ve = scale_exponent(fmaxf(fmaxf(tile_max[1][0], tile_max[1][1]), fmaxf(tile_max[1][2], tile_max[1][3])));
     const float kmul = __builtin_amdgcn_ldexpf(1.0f, ke), vmul = __builtin_amdgcn_ldexpf(1.0f, ve);
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
@@ -600,137 +586,240 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
       for (int pl = 0; pl < PL; ++pl) *reinterpret_cast<uint4*>(tile_v + pl * kPlane + at) = w[pl];
     }
     __syncthreads();
-    if (!active) continue;
+  };
 
-    f32x4 sc[4][2];
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) sc[kb][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int ks = 0; ks < DH / 32; ++ks) {
-        const uint8_t* at = tile_k + (kb * 16 + lr) * kPitch + (ks * 4 + lg) * 16;
-        const f16x8 kh = *reinterpret_cast<const f16x8*>(at);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) sc[kb][r] = mma16(kh, qf[r][ks][0], sc[kb][r]);
-        if constexpr (PL == 2) {
-          const f16x8 kl = *reinterpret_cast<const f16x8*>(at + kPlane);
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            sc[kb][r] = mma16(kl, qf[r][ks][0], sc[kb][r]);
-            sc[kb][r] = mma16(kh, qf[r][ks][PL - 1], sc[kb][r]);
-          }
-        }
-      }
-    }
-    f16x8 pf[2][2][PL];
-    float alpha[2];
+  // This lane's two queries of the 128 entries from i0 on.
+  int entry[2], next_entry[2];
+  float qx[2][KS][8];
+  auto list_at = [&](int i0, int (&to)[2]) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float v = __builtin_amdgcn_ldexpf(sc[kb][r][i], -(qe[r] + ke)) * kLog2e;
-          sc[kb][r][i] = kb * 16 + lg * 4 + i < n ? v : -INFINITY;
-          mx = fmaxf(mx, sc[kb][r][i]);
-        }
-      const float mn = fmaxf(m[r], group_max(mx));
-      const float base = mn == -INFINITY ? 0.0f : mn;
-      alpha[r] = exp2_raw(m[r] - base);
-      m[r] = mn;
-      float sum = 0.0f;
-#pragma unroll
-      for (int kp = 0; kp < 2; ++kp) {
-        float pr[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          pr[i] = exp2_raw(sc[2 * kp + (i >> 2)][r][i & 3] - base);
-          sum += pr[i];
-        }
-        uint4 w[PL];
-        split8<PL>(pr, 1.0f, w);
-#pragma unroll
-        for (int pl = 0; pl < PL; ++pl) pf[r][kp][pl] = __builtin_bit_cast(f16x8, w[pl]);
-      }
-      l[r] = __builtin_fmaf(l[r], alpha[r], sum);
+      const int i = i0 + wave * 32 + r * 16 + lr;
+      to[r] = i < tile.z ? g.list[tile.y + i] : -1;
     }
+  };
+  auto load_q = [&](const int (&of)[2]) {
 #pragma unroll
-    for (int db = 0; db < DH / 16; ++db) {
-      f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    for (int r = 0; r < 2; ++r) {
+      const int row = max(of[r], 0) / p.top, tok = row / p.heads;
+      const T* q =
+          static_cast<const T*>(p.q) + static_cast<size_t>(g.token0 + tok) * p.ldq + (row - tok * p.heads) * dim;
 #pragma unroll
-      for (int kp = 0; kp < 2; ++kp) {
-        const uint8_t* at = tile_v + (kp * 32 + lg * 4 + (lr >> 2)) * kPitch + db * 32 + (lr & 3) * 8;
-        auto frag = [&](const uint8_t* x) {
-          const f16x4 a = lds_read_tr16(x), b = lds_read_tr16(x + 16 * kPitch);
-          return f16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-        };
-        const f16x8 vh = frag(at);
+      for (int ks = 0; ks < KS; ++ks) {
+        const int d = ks * 32 + lg * 8;
+        if (of[r] >= 0 && d < dim) {
+          load8<VEC>(q + d, qx[r][ks]);
+        } else {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) acc[r] = mma16(vh, pf[r][kp][0], acc[r]);
-        if constexpr (PL == 2) {
-          const f16x8 vl = frag(at + kPlane);
+          for (int i = 0; i < 8; ++i) qx[r][ks][i] = 0.0f;
+        }
+      }
+    }
+  };
+  list_at(0, entry);
+  load_q(entry);
+  list_at(128, next_entry);
+  if (keys <= 64) stage(0);
+
+  for (int i0 = 0; i0 < tile.z; i0 += 128) {
+    const bool active = i0 + wave * 32 < tile.z;
+    if (keys <= 64 && !active) break;  // no more barriers, and later entries are none of this wave's
+    f16x8 qf[2][KS][PL];
+    int qe[2];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            acc[r] = mma16(vl, pf[r][kp][0], acc[r]);
-            acc[r] = mma16(vh, pf[r][kp][PL - 1], acc[r]);
+    for (int r = 0; r < 2; ++r) {
+      float amax = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) amax = fmaxf(amax, max8(qx[r][ks]));
+      qe[r] = scale_exponent(group_max(amax));
+      const float mul = __builtin_amdgcn_ldexpf(1.0f, qe[r]);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint4 w[PL];
+        split8<PL>(qx[r][ks], mul, w);
+#pragma unroll
+        for (int pl = 0; pl < PL; ++pl) qf[r][ks][pl] = __builtin_bit_cast(f16x8, w[pl]);
+      }
+    }
+    const int now[2] = {entry[0], entry[1]};
+    entry[0] = next_entry[0];
+    entry[1] = next_entry[1];
+    load_q(entry);
+    list_at(i0 + 256, next_entry);
+
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    f32x4 o[2][DH / 16];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int db = 0; db < DH / 16; ++db) o[r][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    for (int c = 0; c < keys; c += 64) {
+      const int n = min(64, keys - c);
+      if (keys > 64) {
+        stage(c);
+        if (!active) continue;
+      }
+      f32x4 sc[4][2];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) sc[kb][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const uint8_t* at = tile_k + (kb * 16 + lr) * kPitch + (ks * 4 + lg) * 16;
+          const f16x8 kh = *reinterpret_cast<const f16x8*>(at);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) sc[kb][r] = mma16(kh, qf[r][ks][0], sc[kb][r]);
+          if constexpr (PL == 2) {
+            const f16x8 kl = *reinterpret_cast<const f16x8*>(at + kPlane);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              sc[kb][r] = mma16(kl, qf[r][ks][0], sc[kb][r]);
+              sc[kb][r] = mma16(kh, qf[r][ks][PL - 1], sc[kb][r]);
+            }
           }
         }
       }
+      if (n < 64) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+        for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          o[r][db][i] = __builtin_fmaf(o[r][db][i], alpha[r], __builtin_amdgcn_ldexpf(acc[r][i], -ve));
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (kb * 16 + lg * 4 + i >= n) sc[kb][r][i] = -INFINITY;
+      }
+      // Softmax in base 2: the scores' maximum first, then one fused step and an
+      // exponential per score.
+      f16x8 pf[2][2][PL];
+      float alpha[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float unit = __builtin_amdgcn_ldexpf(kLog2e, -(qe[r] + ke));
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[kb][r][i]);
+        const float mn = fmaxf(m[r], group_max(mx) * unit);
+        const float base = mn == -INFINITY ? 0.0f : mn;
+        alpha[r] = exp2_raw(m[r] - base);
+        m[r] = mn;
+        float sum = 0.0f;
+#pragma unroll
+        for (int kp = 0; kp < 2; ++kp) {
+          float pr[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            pr[i] = exp2_raw(__builtin_fmaf(sc[2 * kp + (i >> 2)][r][i & 3], unit, -base));
+            sum += pr[i];
+          }
+          uint4 w[PL];
+          split8<PL>(pr, 1.0f, w);
+#pragma unroll
+          for (int pl = 0; pl < PL; ++pl) pf[r][kp][pl] = __builtin_bit_cast(f16x8, w[pl]);
+        }
+        l[r] = __builtin_fmaf(l[r], alpha[r], sum);
+      }
+      const float vunit = __builtin_amdgcn_ldexpf(1.0f, -ve);
+#pragma unroll
+      for (int db = 0; db < DH / 16; ++db) {
+        f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int kp = 0; kp < 2; ++kp) {
+          const uint8_t* at = tile_v + (kp * 32 + lg * 4 + (lr >> 2)) * kPitch + db * 32 + (lr & 3) * 8;
+          auto frag = [&](const uint8_t* x) {
+            const f16x4 a = lds_read_tr16(x), b = lds_read_tr16(x + 16 * kPitch);
+            return f16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+          };
+          const f16x8 vh = frag(at);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) acc[r] = mma16(vh, pf[r][kp][0], acc[r]);
+          if constexpr (PL == 2) {
+            const f16x8 vl = frag(at + kPlane);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              acc[r] = mma16(vl, pf[r][kp][0], acc[r]);
+              acc[r] = mma16(vh, pf[r][kp][PL - 1], acc[r]);
+            }
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[r][db][i] = __builtin_fmaf(o[r][db][i], alpha[r], acc[r][i] * vunit);
+      }
     }
-  }
 
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const float sum = group_sum(l[r]);
-    if (entry[r] < 0) continue;
-    const size_t at =
-        (static_cast<size_t>(tok[r]) * chunk_heads + head[r] - hk0 * each) * p.top + entry[r] % p.top;
-    if (lg == 0) g.part_ml[at] = make_float2(m[r], sum);
+    for (int r = 0; r < 2; ++r) {
+      const float sum = group_sum(l[r]);
+      if (now[r] < 0) continue;
+      const int row = now[r] / p.top, tok = row / p.heads;
+      const size_t at = (static_cast<size_t>(tok) * chunk_heads + (row - tok * p.heads) - hk0 * each) * p.top +
+                        (now[r] - row * p.top);
+      if (lg == 0) g.part_ml[at] = make_float2(m[r], sum);
 #pragma unroll
-    for (int db = 0; db < DH / 16; ++db)
-      if (db * 16 + lg * 4 < dim) *reinterpret_cast<f32x4*>(g.part_o + at * dim + db * 16 + lg * 4) = o[r][db];
+      for (int db = 0; db < DH / 16; ++db)
+        if (db * 16 + lg * 4 < dim) *reinterpret_cast<f32x4*>(g.part_o + at * dim + db * 16 + lg * 4) = o[r][db];
+    }
   }
 }
 
-// One row's parts, dim / 4 lanes to an entry, joined in the order of its list.
-template <int DT>
+// One row's parts, joined in the order of its list by GL lanes: a lane weighs
+// one entry of every GL and sums four dims of all of them.
+template <int DT, int GL>
 __global__ __launch_bounds__(256) void join_entries_kernel(BlockAttnArgs p, GroupedWork g, int hk0, int hk1) {
   using T = typename ElemOf<DT>::T;
   const int each = p.heads / p.kv_heads, chunk_heads = (hk1 - hk0) * each;
-  const int quads = p.head_dim / 4;
-  const size_t i = blockIdx.x * size_t{256} + threadIdx.x;
-  const size_t row = i / quads;
-  if (row >= static_cast<size_t>(g.tokens) * chunk_heads) return;
-  const int d = static_cast<int>(i % quads) * 4;
+  const int gl = threadIdx.x % GL;
+  const size_t rows = static_cast<size_t>(g.tokens) * chunk_heads;
+  const size_t mine = (blockIdx.x * size_t{256} + threadIdx.x) / GL;
+  const size_t row = mine < rows ? mine : rows - 1;  // lanes past the end keep the shuffles whole
+  const int d = gl * 4, dl = d < p.head_dim ? d : 0;
   const size_t tok = row / chunk_heads;
-  const int head = static_cast<int>(row % chunk_heads) + hk0 * each;
+  const int head = static_cast<int>(row - tok * chunk_heads) + hk0 * each;
   const int* place = g.place + (tok * p.heads + head) * p.top;
   const float2* ml = g.part_ml + row * p.top;
-  const float* o = g.part_o + row * p.top * p.head_dim + d;
-  float m = -INFINITY;
-  for (int e = 0; e < p.top; ++e)
-    if (place[e] >= 0) m = fmaxf(m, ml[e].x);
-  const float base = m == -INFINITY ? 0.0f : m;
-  float sum = 0.0f;
+  const float* o = g.part_o + row * p.top * p.head_dim + dl;
+  float m = -INFINITY, sum = 0.0f;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  for (int e = 0; e < p.top; ++e) {
-    if (place[e] < 0) continue;
-    const float w = exp2_raw(ml[e].x - base);
-    sum = __builtin_fmaf(ml[e].y, w, sum);
-    const f32x4 v = *reinterpret_cast<const f32x4*>(o + static_cast<size_t>(e) * p.head_dim);
+  for (int e0 = 0; e0 < p.top; e0 += GL) {
+    const int n = min(GL, p.top - e0);
+    const bool counts = gl < n && place[e0 + gl] >= 0;
+    const float2 v = counts ? ml[e0 + gl] : make_float2(-INFINITY, 0.0f);
+    float mx = v.x;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = __builtin_fmaf(v[k], w, x[k]);
+    for (int b = 1; b < GL; b *= 2) mx = fmaxf(mx, __shfl_xor(mx, b));
+    const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.0f : mn;
+    const float alpha = exp2_raw(m - base), w = counts ? exp2_raw(v.x - base) : -1.0f;
+    float part = counts ? v.y * w : 0.0f;
+#pragma unroll
+    for (int b = 1; b < GL; b *= 2) part += __shfl_xor(part, b);
+    sum = __builtin_fmaf(sum, alpha, part);
+    m = mn;
+    x *= alpha;
+    const float* at = o + static_cast<size_t>(e0) * p.head_dim;
+    for (int e = 0; e < n; e += 8) {
+      f32x4 y[8];
+      float ws[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        ws[k] = __shfl(w, min(e + k, n - 1), GL);
+        if (e + k >= n) ws[k] = -1.0f;
+        y[k] = *reinterpret_cast<const f32x4*>(at + static_cast<size_t>(min(e + k, n - 1)) * p.head_dim);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = ws[k] != -1.0f ? __builtin_fmaf(y[k][i], ws[k], x[i]) : x[i];
+    }
   }
+  if (mine >= rows || d >= p.head_dim) return;
   T* out = static_cast<T*>(p.out) + ((static_cast<size_t>(g.token0) + tok) * p.heads + head) * p.head_dim + d;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) out[k] = static_cast<T>(sum == 0.0f ? 0.0f : x[k] / sum);
+  for (int i = 0; i < 4; ++i) out[i] = static_cast<T>(sum == 0.0f ? 0.0f : x[i] / sum);
 }
 
 hipError_t launch_block_means(const BlockAttnArgs& p, const SeqTable& t, int type, hipStream_t s) {
@@ -761,7 +850,8 @@ size_t up256(size_t v) { return (v + 255) & ~size_t{255}; }
 // The grouped form's scratch for a plan, laid out from base on.
 GroupedWork grouped_layout(const BlockAttnArgs& p, const BlockAttnPlan& plan, char* base, size_t* bytes) {
   const size_t cells = static_cast<size_t>(p.num_blocks) * p.kv_heads;
-  const size_t entries = static_cast<size_t>(plan.tokens) * p.heads * p.top;
+  const size_t entries = static_cast<size_t>(plan.tokens) * p.heads * p.top, head_entries = entries / p.kv_heads;
+  const size_t head_tiles = head_entries / kTileEntries + std::min<size_t>(p.num_blocks, head_entries);
   const size_t parts = static_cast<size_t>(plan.tokens) * plan.kv_heads * (p.heads / p.kv_heads) * p.top;
   GroupedWork g;
   size_t at = 0;
@@ -770,10 +860,12 @@ GroupedWork grouped_layout(const BlockAttnArgs& p, const BlockAttnPlan& plan, ch
     at += up256(n);
     return q;
   };
+  g.head_entries = static_cast<int>(head_entries);
+  g.head_tiles = static_cast<int>(head_tiles);
   g.counts = reinterpret_cast<int*>(take(cells * 4));
+  g.used = reinterpret_cast<int*>(take(static_cast<size_t>(p.kv_heads) * 4));
   g.first = reinterpret_cast<int*>(take(cells * 4));
-  g.cell_tile = reinterpret_cast<int*>(take((cells + 1) * 4));
-  g.tiles = reinterpret_cast<int4*>(take((entries / kTileEntries + cells + 1) * 16));
+  g.tiles = reinterpret_cast<int4*>(take(head_tiles * p.kv_heads * 16));
   g.place = reinterpret_cast<int*>(take(entries * 4));
   g.list = reinterpret_cast<int*>(take(entries * 4));
   g.part_ml = reinterpret_cast<float2*>(take(parts * 8));
@@ -784,9 +876,25 @@ GroupedWork grouped_layout(const BlockAttnArgs& p, const BlockAttnPlan& plan, ch
 
 template <int DT, int DH>
 hipError_t launch_attention_rows(const BlockAttnArgs& p, const SeqTable& t, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(p.rows) * p.heads;
-  attention_rows_kernel<DT, DH><<<grid, 64 * (p.top < 8 ? p.top : 8), 0, s>>>(p, t);
+  const unsigned grid = static_cast<unsigned>(p.rows) * p.heads, block = 64 * (p.top < 8 ? p.top : 8);
+  if (p.vec_kv)
+    attention_rows_kernel<DT, DH, true><<<grid, block, 0, s>>>(p, t);
+  else
+    attention_rows_kernel<DT, DH, false><<<grid, block, 0, s>>>(p, t);
   return hipGetLastError();
+}
+
+template <int DT>
+void launch_join(const BlockAttnArgs& p, const GroupedWork& g, int h0, int h1, size_t rows, hipStream_t s) {
+  const auto grid = [&](int lanes) { return static_cast<unsigned>((rows * lanes + 255) / 256); };
+  if (p.head_dim <= 16)
+    join_entries_kernel<DT, 4><<<grid(4), 256, 0, s>>>(p, g, h0, h1);
+  else if (p.head_dim <= 32)
+    join_entries_kernel<DT, 8><<<grid(8), 256, 0, s>>>(p, g, h0, h1);
+  else if (p.head_dim <= 64)
+    join_entries_kernel<DT, 16><<<grid(16), 256, 0, s>>>(p, g, h0, h1);
+  else
+    join_entries_kernel<DT, 32><<<grid(32), 256, 0, s>>>(p, g, h0, h1);
 }
 
 template <int DT, int DH>
@@ -798,24 +906,25 @@ hipError_t launch_attention_cells(const BlockAttnArgs& p, const SeqTable& t, con
   for (int t0 = 0; t0 < p.rows; t0 += plan.tokens) {
     g.token0 = t0;
     g.tokens = p.rows - t0 < plan.tokens ? p.rows - t0 : plan.tokens;
-    const size_t entries = static_cast<size_t>(g.tokens) * p.heads * p.top;
-    hipError_t e = launch_fill_f32(reinterpret_cast<float*>(g.counts), cells, 0.0f, s);  // integer zeros
+    const hipError_t e = launch_fill_f32(reinterpret_cast<float*>(g.counts), cells, 0.0f, s);  // integer zeros
     if (e != hipSuccess) return e;
     const int per = kCountEntries / p.top;
     const unsigned groups = static_cast<unsigned>((g.tokens + per - 1) / per) * p.heads;
-    count_entries_kernel<<<groups, kCountThreads, 0, s>>>(p, t, g, per);
-    scan_cells_kernel<<<1, kScanThreads, 0, s>>>(g, cells);
-    const unsigned sgrid = static_cast<unsigned>(entries / 256 + 1 < 16384 ? entries / 256 + 1 : 16384);
-    scatter_entries_kernel<<<sgrid, 256, 0, s>>>(p, t, g);
-    for (int h0 = 0; h0 < p.kv_heads; h0 += plan.kv_heads) {
-      const int h1 = h0 + plan.kv_heads < p.kv_heads ? h0 + plan.kv_heads : p.kv_heads;
-      const size_t rows = static_cast<size_t>(g.tokens) * (h1 - h0) * each;
-      const size_t tiles = rows * p.top / kTileEntries + static_cast<size_t>(h1 - h0) * p.num_blocks;
-      attention_cells_kernel<DT, DH><<<static_cast<unsigned>(tiles), 256, 0, s>>>(p, t, g, h0, h1);
-      join_entries_kernel<DT><<<static_cast<unsigned>((rows * (p.head_dim / 4) + 255) / 256), 256, 0, s>>>(p, g, h0, h1);
+    count_entries_kernel<<<groups, kCountThreads, 0, s>>>(p, t, g);
+    place_cells_kernel<<<p.kv_heads, kPlaceThreads, 0, s>>>(p, g);
+    scatter_entries_kernel<<<groups, kCountThreads, 0, s>>>(p, t, g);
+    for (int h0 = 0, heads = plan.kv_heads; h0 < p.kv_heads; h0 += heads) {
+      while (h0 + heads > p.kv_heads) heads /= 2;
+      const int h1 = h0 + heads, xcds = 8 / heads;
+      const unsigned grid = static_cast<unsigned>((g.head_tiles + xcds - 1) / xcds) * 8;
+      if (p.vec_kv && p.vec_q)
+        attention_cells_kernel<DT, DH, true><<<grid, 256, 0, s>>>(p, t, g, h0, h1);
+      else
+        attention_cells_kernel<DT, DH, false><<<grid, 256, 0, s>>>(p, t, g, h0, h1);
+      launch_join<DT>(p, g, h0, h1, static_cast<size_t>(g.tokens) * (h1 - h0) * each, s);
     }
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    const hipError_t done = hipGetLastError();
+    if (done != hipSuccess) return done;
   }
   return hipSuccess;
 }
@@ -843,7 +952,8 @@ BlockAttnPlan attention_blocks_plan(const BlockAttnArgs& p) {
   // Entry numbers are 32-bit, and lists of 2^26 entries take half a gigabyte.
   plan.tokens = static_cast<int>(std::min<size_t>(p.rows, std::max<size_t>(1, (size_t{1} << 26) / row_entries)));
   const size_t head_bytes = static_cast<size_t>(plan.tokens) * (p.heads / p.kv_heads) * p.top * (p.head_dim * 4 + 8);
-  plan.kv_heads = static_cast<int>(std::min<size_t>(p.kv_heads, std::max<size_t>(1, kPartBytes / head_bytes)));
+  plan.kv_heads = 8;
+  while (plan.kv_heads > 1 && (plan.kv_heads > p.kv_heads || plan.kv_heads * head_bytes > kPartBytes)) plan.kv_heads /= 2;
   grouped_layout(p, plan, nullptr, &plan.scratch_bytes);
   return plan;
 }
