@@ -18,24 +18,43 @@ namespace esm_gfx950 {
 
 namespace {
 
-// Parts of the grouped attention that are in flight between the pass that
-// writes them and the one that joins them: what the 256 MB memory-side cache
-// holds beside the keys.
+// Parts that the grouped attention has in flight between the pass that writes
+// them and the one that joins them, some key heads at a time: no more than the
+// 256 MB memory-side cache holds beside the keys (joining 138 MB took 24 us,
+// 692 MB at once 175).
 constexpr size_t kPartBytes = size_t{160} << 20;
+
+// Division of 0 <= n < 2^31 by a launch's constant, in three instructions: with
+// s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1, n / d is
+// (floor(n m / 2^32) + n) / 2^s (Granlund and Montgomery, 1994).
+struct Divisor {
+  uint32_t mul = 0, shift = 0;
+  int d = 1;
+  Divisor() = default;
+  explicit Divisor(int by) : d(by) {
+    while ((uint64_t{1} << shift) < static_cast<uint64_t>(by)) ++shift;
+    mul = static_cast<uint32_t>(((uint64_t{1} << 32) * ((uint64_t{1} << shift) - by)) / by + 1);
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
+  }
+};
 
 // The grouped attention's device scratch (attention, block by block).
 struct GroupedWork {
   int token0 = 0, tokens = 0;  // the tokens in hand
+  Divisor by_top, by_heads;
   int head_entries = 0;        // entries of a key head, counting or not
-  int head_tiles = 0;          // most tiles of a key head
+  int group_heads = 0;         // key heads that are attended to together
+  int group_tiles = 0;         // most tiles of such a group
   int* counts = nullptr;       // [cells] entries
-  int* used = nullptr;         // [kv_heads] tiles of a key head
+  int* used = nullptr;         // [groups] tiles of a group (behind counts)
   int* first = nullptr;        // [cells] first entry in list
-  int4* tiles = nullptr;       // [kv_heads, head_tiles] (cell, first entry, entries, -)
+  int4* tiles = nullptr;       // [groups, group_tiles] (cell, first entry, entries, -), each key head's together
   int* place = nullptr;        // [entries] place in its cell, -1: does not count
   int* list = nullptr;         // [entries] by cell
   float2* part_ml = nullptr;   // [entries of the heads in hand] maximum (base 2) and sum
-  float* part_o = nullptr;     // [.., head_dim]
+  float* part_o = nullptr;     // [.., padded head_dim]; one entry more takes what belongs to none
 };
 
 template <int DT>
@@ -54,7 +73,7 @@ struct ElemOf<kTypeBF16> {
 };
 
 struct Seq {
-  int q0, k0, k1, b0, b1;
+  int k0, k1, b0, b1;
 };
 
 __device__ __forceinline__ int table_at(const SeqTable& t, const int* inl, int which, int i) {
@@ -76,8 +95,8 @@ __device__ __forceinline__ int seq_of(const SeqTable& t, const int* inl, int whi
 }
 
 __device__ __forceinline__ Seq seq_at(const SeqTable& t, int b) {
-  return Seq{table_at(t, t.cu_q, 0, b), table_at(t, t.cu_k, 1, b), table_at(t, t.cu_k, 1, b + 1),
-             table_at(t, t.cb, 2, b), table_at(t, t.cb, 2, b + 1)};
+  return Seq{table_at(t, t.cu_k, 1, b), table_at(t, t.cu_k, 1, b + 1), table_at(t, t.cb, 2, b),
+             table_at(t, t.cb, 2, b + 1)};
 }
 
 // Order-preserving key of a score: larger scores have larger keys, NaN counts
@@ -202,10 +221,16 @@ __device__ __forceinline__ void load8(const T* x, float (&out)[8]) {
   for (int i = 0; i < 8; ++i) out[i] = static_cast<float>(v[i]);
 }
 
-__device__ __forceinline__ float max8(const float (&x)[8]) {
+// The largest of three, in one instruction (fmaxf quiets its operands first).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float max8(const float (&x)[8]) {  // of the magnitudes
   float m = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
+  for (int i = 0; i < 8; i += 2) asm("v_max3_f32 %0, |%1|, |%2|, %0" : "+v"(m) : "v"(x[i]), "v"(x[i + 1]));
   return m;
 }
 
@@ -405,32 +430,40 @@ __global__ __launch_bounds__(kCountThreads) void count_entries_kernel(BlockAttnA
   const EntryRange r = entry_range(p, g);
   int* cells = g.counts + static_cast<size_t>(r.hk) * p.num_blocks;
   const bool lds = p.num_blocks <= kCountBlocks;
+  // Every load first: entry u * 256 + thread of the range, and the one before it.
+  int block[kCountPer], before[kCountPer], tok[kCountPer];
+  const int* lists = p.blocks + (static_cast<size_t>(g.token0 + r.first) * p.heads + r.head) * p.top;
+#pragma unroll
+  for (int u = 0; u < kCountPer; ++u) {
+    const int i = min(u * kCountThreads + static_cast<int>(threadIdx.x), r.entries - 1);
+    tok[u] = g.by_top(i);
+    const int e = i - tok[u] * p.top;
+    const int* at = lists + static_cast<size_t>(tok[u]) * p.heads * p.top + e;
+    block[u] = *at;
+    before[u] = e > 0 ? at[-1] : 0x80000000;
+  }
   for (int i = threadIdx.x; lds && i < p.num_blocks; i += kCountThreads) hist[i] = 0;
-  for (int i = threadIdx.x; i < r.entries / p.top; i += kCountThreads) unsorted[i] = 0;
+  for (int i = threadIdx.x, n = g.by_top(r.entries); i < n; i += kCountThreads) unsorted[i] = 0;
   __syncthreads();
   // A list that ascends and then ends in negatives, as the selection's do, has
   // no repeats.
-  int block[kCountPer], place[kCountPer];
 #pragma unroll
   for (int u = 0; u < kCountPer; ++u) {
-    const int i = u * kCountThreads + threadIdx.x, tok = i / p.top, e = i - tok * p.top;
-    block[u] = -1;
-    if (i >= r.entries) continue;
-    const int* list = p.blocks + (static_cast<size_t>(g.token0 + r.first + tok) * p.heads + r.head) * p.top;
-    const int j = list[e];
-    if (e > 0 && j >= 0 && (list[e - 1] < 0 || j <= list[e - 1])) unsorted[tok] = 1;
-    block[u] = j;
+    if (u * kCountThreads + static_cast<int>(threadIdx.x) >= r.entries) block[u] = -1;
+    if (block[u] >= 0 && before[u] != static_cast<int>(0x80000000) && (before[u] < 0 || block[u] <= before[u]))
+      unsorted[tok[u]] = 1;
   }
   __syncthreads();
+  int place[kCountPer];
 #pragma unroll
   for (int u = 0; u < kCountPer; ++u) {
-    const int i = u * kCountThreads + threadIdx.x, tok = i / p.top, e = i - tok * p.top;
     place[u] = -1;
     if (block[u] < 0) continue;
-    const Seq s = seq_at(t, seq_of(t, t.cu_q, 0, g.token0 + r.first + tok));
+    const Seq s = seq_at(t, seq_of(t, t.cu_q, 0, g.token0 + r.first + tok[u]));
     bool counts = block[u] < s.b1 - s.b0;
-    if (unsorted[tok]) {
-      const int* list = p.blocks + (static_cast<size_t>(g.token0 + r.first + tok) * p.heads + r.head) * p.top;
+    if (unsorted[tok[u]]) {
+      const int* list = lists + static_cast<size_t>(tok[u]) * p.heads * p.top;
+      const int e = u * kCountThreads + threadIdx.x - tok[u] * p.top;
       for (int k = 0; k < e; ++k) counts &= list[k] != block[u];
     }
     if (!counts) continue;
@@ -447,24 +480,39 @@ __global__ __launch_bounds__(kCountThreads) void count_entries_kernel(BlockAttnA
   }
 #pragma unroll
   for (int u = 0; u < kCountPer; ++u) {
-    const int i = u * kCountThreads + threadIdx.x, tok = i / p.top, e = i - tok * p.top;
+    const int i = u * kCountThreads + threadIdx.x;
     if (i >= r.entries) continue;
     if (lds && place[u] >= 0) place[u] += hist[block[u]];
-    g.place[(static_cast<size_t>(r.first + tok) * p.heads + r.head) * p.top + e] = place[u];
+    g.place[(static_cast<size_t>(r.first + tok[u]) * p.heads + r.head) * p.top + (i - tok[u] * p.top)] = place[u];
   }
 }
 
 // One workgroup per key head: running sums over its cells' entries and tiles give
-// every cell its stretch of the list and its tiles. (One thread per cell with
-// atomics on the head's two totals took 29 us for 129 blocks of 20 heads.)
+// every cell its stretch of the list and its tiles, behind the tiles of whichever
+// heads of the group came before (nothing depends on their order). One thread per
+// cell with atomics on the head's two totals took 29 us for 129 blocks of 20 heads.
 constexpr int kPlaceThreads = 512;
 __global__ __launch_bounds__(kPlaceThreads) void place_cells_kernel(BlockAttnArgs p, GroupedWork g) {
   __shared__ int sums[2][kPlaceThreads / 64];
-  const int hk = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int at0 = hk * g.head_entries, tile0 = hk * g.head_tiles;
+  __shared__ int base;
+  const int hk = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = hk / g.group_heads;
+  auto cell_tiles = [](int n) { return (n + kTileEntries - 1) / kTileEntries; };
+  int mine = 0;
+  for (int b = threadIdx.x; b < p.num_blocks; b += kPlaceThreads) mine += cell_tiles(g.counts[hk * p.num_blocks + b]);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) mine += __shfl_xor(mine, d);
+  if (lane == 0) sums[0][wave] = mine;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int n = 0;
+    for (int w = 0; w < kPlaceThreads / 64; ++w) n += sums[0][w];
+    base = group * g.group_tiles + atomicAdd(&g.used[group], n);
+  }
+  __syncthreads();
+  int at0 = hk * g.head_entries, tile0 = base;
   for (int c0 = 0; c0 < p.num_blocks; c0 += kPlaceThreads) {
     const int block = c0 + threadIdx.x, c = hk * p.num_blocks + block;
-    const int n = block < p.num_blocks ? g.counts[c] : 0, tiles = (n + kTileEntries - 1) / kTileEntries;
+    const int n = block < p.num_blocks ? g.counts[c] : 0, tiles = cell_tiles(n);
     int n_to = n, tiles_to = tiles;  // sums over the wave's lanes up to this one
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -490,22 +538,28 @@ __global__ __launch_bounds__(kPlaceThreads) void place_cells_kernel(BlockAttnArg
       g.tiles[tile + i] = make_int4(c, at + i * kTileEntries, min(kTileEntries, n - i * kTileEntries), 0);
     __syncthreads();
   }
-  if (threadIdx.x == 0) g.used[hk] = tile0 - hk * g.head_tiles;
 }
 
 __global__ __launch_bounds__(kCountThreads) void scatter_entries_kernel(BlockAttnArgs p, SeqTable t, GroupedWork g) {
   const EntryRange r = entry_range(p, g);
+  int at[kCountPer], place[kCountPer], block[kCountPer];
 #pragma unroll
   for (int u = 0; u < kCountPer; ++u) {
-    const int i = u * kCountThreads + threadIdx.x, tok = i / p.top, e = i - tok * p.top;
-    if (i >= r.entries) continue;
-    const size_t at = (static_cast<size_t>(r.first + tok) * p.heads + r.head) * p.top + e;
-    const int place = g.place[at];
-    if (place < 0) continue;
-    const int j = seq_at(t, seq_of(t, t.cu_q, 0, g.token0 + r.first + tok)).b0 +
-                  p.blocks[static_cast<size_t>(g.token0) * p.heads * p.top + at];
-    g.list[g.first[r.hk * p.num_blocks + j] + place] = static_cast<int>(at);
+    const int i = min(u * kCountThreads + static_cast<int>(threadIdx.x), r.entries - 1), tok = g.by_top(i);
+    at[u] = ((r.first + tok) * p.heads + r.head) * p.top + (i - tok * p.top);
+    place[u] = g.place[at[u]];
+    block[u] = p.blocks[static_cast<size_t>(g.token0) * p.heads * p.top + at[u]] +
+               seq_at(t, seq_of(t, t.cu_q, 0, g.token0 + r.first + tok)).b0;
   }
+  int first[kCountPer];
+#pragma unroll
+  for (int u = 0; u < kCountPer; ++u) {
+    if (u * kCountThreads + static_cast<int>(threadIdx.x) >= r.entries) place[u] = -1;
+    first[u] = place[u] >= 0 ? g.first[r.hk * p.num_blocks + block[u]] : 0;
+  }
+#pragma unroll
+  for (int u = 0; u < kCountPer; ++u)
+    if (place[u] >= 0) g.list[first[u] + place[u]] = at[u];
 }
 
 // One workgroup per tile of up to 512 entries of a cell, 32 at a time to a wave.
@@ -516,7 +570,9 @@ __global__ __launch_bounds__(kCountThreads) void scatter_entries_kernel(BlockAtt
 // the tile's entries on their own, the next ones' queries on their way. S^T =
 // K Q^T leaves a lane the scores of one query with keys 4 lg .. + 4 of every 16,
 // which is the operand of O^T = V^T P^T as it stands.
-template <int DT, int DH, bool VEC>
+//
+// ONE: no block is longer than 64 keys.
+template <int DT, int DH, bool VEC, bool ONE>
 __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, SeqTable t, GroupedWork g, int hk0,
                                                               int hk1) {
   using T = typename ElemOf<DT>::T;
@@ -529,17 +585,18 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
   __shared__ float tile_max[2][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int lr = lane & 15, lg = lane >> 4;
-  // Workgroup i runs on XCD i % 8, and each XCD has its own L2: the hk1 - hk0 (1,
-  // 2, 4 or 8) key heads in hand get as many XCDs each, whose L2s then hold that
-  // head's queries.
-  const int xcds = 8 / (hk1 - hk0), xcd = blockIdx.x % 8;
-  const int hk = hk0 + xcd / xcds, nth = blockIdx.x / 8 * xcds + xcd % xcds;
-  if (nth >= g.used[hk]) return;
-  const int4 tile = g.tiles[hk * g.head_tiles + nth];
-  const int block = tile.x - hk * p.num_blocks, dim = p.head_dim;
+  // Workgroup i runs on XCD i % 8, and each XCD has its own L2: an XCD takes an
+  // eighth of the tiles one after the other, two or three key heads' of 20, and
+  // finds their queries in its L2.
+  const int group = hk0 / g.group_heads, tiles = g.used[group], per = (tiles + 7) / 8;
+  const int nth = blockIdx.x % 8 * per + blockIdx.x / 8;
+  if (static_cast<int>(blockIdx.x / 8) >= per || nth >= tiles) return;
+  const int4 tile = g.tiles[group * g.group_tiles + nth];
+  const int hk = tile.x / p.num_blocks, block = tile.x - hk * p.num_blocks, dim = p.head_dim;
   const Seq s = seq_at(t, seq_of(t, t.cb, 2, block));
   const int key0 = s.k0 + (block - s.b0) * p.block_size, keys = min(p.block_size, s.k1 - key0);
   const int each = p.heads / p.kv_heads, chunk_heads = (hk1 - hk0) * each;
+  const int no_part = g.tokens * chunk_heads * p.top;
 
   // Loads the 64 keys from key0 + c on, and their values, into LDS.
   int ke = 0, ve = 0;
@@ -588,42 +645,41 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
     __syncthreads();
   };
 
-  // This lane's two queries of the 128 entries from i0 on.
-  int entry[2], next_entry[2];
+  // This lane's two queries of the 128 entries from i0 on, and where their parts go.
+  int entry[2], next_entry[2], part[2];
   float qx[2][KS][8];
   auto list_at = [&](int i0, int (&to)[2]) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int i = i0 + wave * 32 + r * 16 + lr;
-      to[r] = i < tile.z ? g.list[tile.y + i] : -1;
+      const int i = i0 + wave * 32 + r * 16 + lr, e = g.list[tile.y + min(i, tile.z - 1)];
+      to[r] = i < tile.z ? e : -1;
     }
   };
+  // Loads and stores without conditions, so that a wait for the next queries
+  // counts the stores behind them instead of waiting for those too: lanes without
+  // an entry read the first query and write past the last part, and dims past the
+  // head read its first ones (the keys are zero there).
   auto load_q = [&](const int (&of)[2]) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int row = max(of[r], 0) / p.top, tok = row / p.heads;
-      const T* q =
-          static_cast<const T*>(p.q) + static_cast<size_t>(g.token0 + tok) * p.ldq + (row - tok * p.heads) * dim;
+      const int row = g.by_top(max(of[r], 0)), tok = g.by_heads(row), head = row - tok * p.heads;
+      part[r] = of[r] < 0 ? no_part : (tok * chunk_heads + head - hk0 * each) * p.top + (of[r] - row * p.top);
+      const T* q = static_cast<const T*>(p.q) + static_cast<size_t>(g.token0 + tok) * p.ldq + head * dim;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int d = ks * 32 + lg * 8;
-        if (of[r] >= 0 && d < dim) {
-          load8<VEC>(q + d, qx[r][ks]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) qx[r][ks][i] = 0.0f;
-        }
+        load8<VEC>(q + (d < dim ? d : 0), qx[r][ks]);
       }
     }
   };
   list_at(0, entry);
   load_q(entry);
   list_at(128, next_entry);
-  if (keys <= 64) stage(0);
+  if (ONE) stage(0);
 
   for (int i0 = 0; i0 < tile.z; i0 += 128) {
     const bool active = i0 + wave * 32 < tile.z;
-    if (keys <= 64 && !active) break;  // no more barriers, and later entries are none of this wave's
+    if (ONE && !active) break;  // no more barriers, and later entries are none of this wave's
     f16x8 qf[2][KS][PL];
     int qe[2];
 #pragma unroll
@@ -641,7 +697,7 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
         for (int pl = 0; pl < PL; ++pl) qf[r][ks][pl] = __builtin_bit_cast(f16x8, w[pl]);
       }
     }
-    const int now[2] = {entry[0], entry[1]};
+    const int now[2] = {part[0], part[1]};
     entry[0] = next_entry[0];
     entry[1] = next_entry[1];
     load_q(entry);
@@ -654,9 +710,9 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
 #pragma unroll
       for (int db = 0; db < DH / 16; ++db) o[r][db] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    for (int c = 0; c < keys; c += 64) {
+    for (int c = 0; c < (ONE ? 1 : keys); c += 64) {
       const int n = min(64, keys - c);
-      if (keys > 64) {
+      if constexpr (!ONE) {
         stage(c);
         if (!active) continue;
       }
@@ -699,9 +755,10 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
         const float unit = __builtin_amdgcn_ldexpf(kLog2e, -(qe[r] + ke));
         float mx = -INFINITY;
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[kb][r][i]);
+        for (int kb = 0; kb < 4; ++kb) {
+          mx = max3(sc[kb][r][0], sc[kb][r][1], mx);
+          mx = max3(sc[kb][r][2], sc[kb][r][3], mx);
+        }
         const float mn = fmaxf(m[r], group_max(mx) * unit);
         const float base = mn == -INFINITY ? 0.0f : mn;
         alpha[r] = exp2_raw(m[r] - base);
@@ -748,21 +805,19 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
 #pragma unroll
         for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[r][db][i] = __builtin_fmaf(o[r][db][i], alpha[r], acc[r][i] * vunit);
+          for (int i = 0; i < 4; ++i)
+            o[r][db][i] = ONE ? acc[r][i] * vunit : __builtin_fmaf(o[r][db][i], alpha[r], acc[r][i] * vunit);
       }
     }
 
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const float sum = group_sum(l[r]);
-      if (now[r] < 0) continue;
-      const int row = now[r] / p.top, tok = row / p.heads;
-      const size_t at = (static_cast<size_t>(tok) * chunk_heads + (row - tok * p.heads) - hk0 * each) * p.top +
-                        (now[r] - row * p.top);
-      if (lg == 0) g.part_ml[at] = make_float2(m[r], sum);
+      const size_t at = now[r];
+      g.part_ml[at] = make_float2(m[r], sum);  // the same from all four lanes
 #pragma unroll
       for (int db = 0; db < DH / 16; ++db)
-        if (db * 16 + lg * 4 < dim) *reinterpret_cast<f32x4*>(g.part_o + at * dim + db * 16 + lg * 4) = o[r][db];
+        *reinterpret_cast<f32x4*>(g.part_o + at * DH + db * 16 + lg * 4) = o[r][db];
     }
   }
 }
@@ -782,7 +837,8 @@ __global__ __launch_bounds__(256) void join_entries_kernel(BlockAttnArgs p, Grou
   const int head = static_cast<int>(row - tok * chunk_heads) + hk0 * each;
   const int* place = g.place + (tok * p.heads + head) * p.top;
   const float2* ml = g.part_ml + row * p.top;
-  const float* o = g.part_o + row * p.top * p.head_dim + dl;
+  constexpr int kStride = GL * 4 < 32 ? 32 : GL * 4;  // the parts' padded head_dim
+  const float* o = g.part_o + row * p.top * kStride + dl;
   float m = -INFINITY, sum = 0.0f;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
   for (int e0 = 0; e0 < p.top; e0 += GL) {
@@ -800,7 +856,7 @@ __global__ __launch_bounds__(256) void join_entries_kernel(BlockAttnArgs p, Grou
     sum = __builtin_fmaf(sum, alpha, part);
     m = mn;
     x *= alpha;
-    const float* at = o + static_cast<size_t>(e0) * p.head_dim;
+    const float* at = o + static_cast<size_t>(e0) * kStride;
     for (int e = 0; e < n; e += 8) {
       f32x4 y[8];
       float ws[8];
@@ -808,7 +864,7 @@ __global__ __launch_bounds__(256) void join_entries_kernel(BlockAttnArgs p, Grou
       for (int k = 0; k < 8; ++k) {
         ws[k] = __shfl(w, min(e + k, n - 1), GL);
         if (e + k >= n) ws[k] = -1.0f;
-        y[k] = *reinterpret_cast<const f32x4*>(at + static_cast<size_t>(min(e + k, n - 1)) * p.head_dim);
+        y[k] = *reinterpret_cast<const f32x4*>(at + static_cast<size_t>(min(e + k, n - 1)) * kStride);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k)
@@ -847,11 +903,14 @@ namespace {
 
 size_t up256(size_t v) { return (v + 255) & ~size_t{255}; }
 
+int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+
 // The grouped form's scratch for a plan, laid out from base on.
 GroupedWork grouped_layout(const BlockAttnArgs& p, const BlockAttnPlan& plan, char* base, size_t* bytes) {
   const size_t cells = static_cast<size_t>(p.num_blocks) * p.kv_heads;
   const size_t entries = static_cast<size_t>(plan.tokens) * p.heads * p.top, head_entries = entries / p.kv_heads;
   const size_t head_tiles = head_entries / kTileEntries + std::min<size_t>(p.num_blocks, head_entries);
+  const int groups = (p.kv_heads + plan.kv_heads - 1) / plan.kv_heads;
   const size_t parts = static_cast<size_t>(plan.tokens) * plan.kv_heads * (p.heads / p.kv_heads) * p.top;
   GroupedWork g;
   size_t at = 0;
@@ -860,16 +919,19 @@ GroupedWork grouped_layout(const BlockAttnArgs& p, const BlockAttnPlan& plan, ch
     at += up256(n);
     return q;
   };
+  g.by_top = Divisor(p.top);
+  g.by_heads = Divisor(p.heads);
   g.head_entries = static_cast<int>(head_entries);
-  g.head_tiles = static_cast<int>(head_tiles);
-  g.counts = reinterpret_cast<int*>(take(cells * 4));
-  g.used = reinterpret_cast<int*>(take(static_cast<size_t>(p.kv_heads) * 4));
+  g.group_heads = plan.kv_heads;
+  g.group_tiles = static_cast<int>(head_tiles * plan.kv_heads);
+  g.counts = reinterpret_cast<int*>(take((cells + groups) * 4));
+  g.used = g.counts ? g.counts + cells : nullptr;
   g.first = reinterpret_cast<int*>(take(cells * 4));
-  g.tiles = reinterpret_cast<int4*>(take(head_tiles * p.kv_heads * 16));
+  g.tiles = reinterpret_cast<int4*>(take(head_tiles * plan.kv_heads * groups * 16));
   g.place = reinterpret_cast<int*>(take(entries * 4));
   g.list = reinterpret_cast<int*>(take(entries * 4));
-  g.part_ml = reinterpret_cast<float2*>(take(parts * 8));
-  g.part_o = reinterpret_cast<float*>(take(parts * p.head_dim * 4));
+  g.part_ml = reinterpret_cast<float2*>(take((parts + 1) * 8));
+  g.part_o = reinterpret_cast<float*>(take((parts + 1) * padded_dim(p.head_dim) * 4));
   *bytes = at;
   return g;
 }
@@ -906,21 +968,25 @@ hipError_t launch_attention_cells(const BlockAttnArgs& p, const SeqTable& t, con
   for (int t0 = 0; t0 < p.rows; t0 += plan.tokens) {
     g.token0 = t0;
     g.tokens = p.rows - t0 < plan.tokens ? p.rows - t0 : plan.tokens;
-    const hipError_t e = launch_fill_f32(reinterpret_cast<float*>(g.counts), cells, 0.0f, s);  // integer zeros
+    const int groups = (p.kv_heads + g.group_heads - 1) / g.group_heads;
+    // Integer zeros for counts and used.
+    const hipError_t e = launch_fill_f32(reinterpret_cast<float*>(g.counts), cells + groups, 0.0f, s);
     if (e != hipSuccess) return e;
     const int per = kCountEntries / p.top;
-    const unsigned groups = static_cast<unsigned>((g.tokens + per - 1) / per) * p.heads;
-    count_entries_kernel<<<groups, kCountThreads, 0, s>>>(p, t, g);
+    const unsigned ranges = static_cast<unsigned>((g.tokens + per - 1) / per) * p.heads;
+    count_entries_kernel<<<ranges, kCountThreads, 0, s>>>(p, t, g);
     place_cells_kernel<<<p.kv_heads, kPlaceThreads, 0, s>>>(p, g);
-    scatter_entries_kernel<<<groups, kCountThreads, 0, s>>>(p, t, g);
-    for (int h0 = 0, heads = plan.kv_heads; h0 < p.kv_heads; h0 += heads) {
-      while (h0 + heads > p.kv_heads) heads /= 2;
-      const int h1 = h0 + heads, xcds = 8 / heads;
-      const unsigned grid = static_cast<unsigned>((g.head_tiles + xcds - 1) / xcds) * 8;
-      if (p.vec_kv && p.vec_q)
-        attention_cells_kernel<DT, DH, true><<<grid, 256, 0, s>>>(p, t, g, h0, h1);
+    scatter_entries_kernel<<<ranges, kCountThreads, 0, s>>>(p, t, g);
+    for (int h0 = 0; h0 < p.kv_heads; h0 += g.group_heads) {
+      const int h1 = std::min(h0 + g.group_heads, p.kv_heads);
+      const unsigned grid = static_cast<unsigned>(g.group_tiles + 7) / 8 * 8;
+      const bool vec = p.vec_kv && p.vec_q;
+      if (p.block_size <= 64)
+        vec ? attention_cells_kernel<DT, DH, true, true><<<grid, 256, 0, s>>>(p, t, g, h0, h1)
+            : attention_cells_kernel<DT, DH, false, true><<<grid, 256, 0, s>>>(p, t, g, h0, h1);
       else
-        attention_cells_kernel<DT, DH, false><<<grid, 256, 0, s>>>(p, t, g, h0, h1);
+        vec ? attention_cells_kernel<DT, DH, true, false><<<grid, 256, 0, s>>>(p, t, g, h0, h1)
+            : attention_cells_kernel<DT, DH, false, false><<<grid, 256, 0, s>>>(p, t, g, h0, h1);
       launch_join<DT>(p, g, h0, h1, static_cast<size_t>(g.tokens) * (h1 - h0) * each, s);
     }
     const hipError_t done = hipGetLastError();
@@ -951,9 +1017,9 @@ BlockAttnPlan attention_blocks_plan(const BlockAttnArgs& p) {
   if (!plan.grouped) return plan;
   // Entry numbers are 32-bit, and lists of 2^26 entries take half a gigabyte.
   plan.tokens = static_cast<int>(std::min<size_t>(p.rows, std::max<size_t>(1, (size_t{1} << 26) / row_entries)));
-  const size_t head_bytes = static_cast<size_t>(plan.tokens) * (p.heads / p.kv_heads) * p.top * (p.head_dim * 4 + 8);
-  plan.kv_heads = 8;
-  while (plan.kv_heads > 1 && (plan.kv_heads > p.kv_heads || plan.kv_heads * head_bytes > kPartBytes)) plan.kv_heads /= 2;
+  const size_t head_bytes =
+      static_cast<size_t>(plan.tokens) * (p.heads / p.kv_heads) * p.top * (padded_dim(p.head_dim) * 4 + 8);
+  plan.kv_heads = static_cast<int>(std::min<size_t>(p.kv_heads, std::max<size_t>(1, kPartBytes / head_bytes)));
   grouped_layout(p, plan, nullptr, &plan.scratch_bytes);
   return plan;
 }
