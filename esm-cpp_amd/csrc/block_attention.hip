@@ -80,7 +80,7 @@ __device__ __forceinline__ int table_at(const SeqTable& t, const int* inl, int w
   return t.dev ? t.dev[which * (t.batch + 1) + i] : inl[i];
 }
 
-// The sequence whose range of `which` (0 cu_q, 2 cb) holds x: the last one that
+// The sequence whose range of `which` (0 cu_q, 2 cb, 3 ct) holds x: the last one that
 // starts at or before x (empty ranges hold nothing).
 __device__ __forceinline__ int seq_of(const SeqTable& t, const int* inl, int which, int x) {
   int lo = 0, hi = t.batch;  // at(lo) <= x < at(hi)
@@ -125,10 +125,208 @@ __global__ __launch_bounds__(256) void block_means_kernel(BlockAttnArgs p, SeqTa
   }
 }
 
-// One wave per (query, head). Scores in 64 bits, kept as order-preserving keys
-// in LDS, kSelChunk blocks at a time behind the `top` kept from the chunks
-// before; the top-th largest key is found bit by bit with counts by ballot, and
-// what is above it (and equal to it, lowest index first) stays in order.
+namespace {
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+// Order-preserving 32-bit key of a score's fp32 rounding, never 0.
+__device__ __forceinline__ uint32_t score_key32(double s) {
+  if (s != s) s = -INFINITY;
+  const uint32_t u = __float_as_uint(static_cast<float>(s + 0.0) + 0.0f);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+// One wave: of the n 64-bit keys, the `want` largest (ties to the lowest index),
+// handed to take(position, index, key) in ascending order of their indices.
+// Their smallest is found bit by bit with counts by ballot.
+template <class F>
+__device__ __forceinline__ void take_largest(const uint64_t* keys, int n, int want, F take) {
+  const int lane = threadIdx.x & 63;
+  uint64_t thr = 0;
+  for (int bit = 63; bit >= 0; --bit) {
+    const uint64_t cand = thr | (uint64_t{1} << bit);
+    int count = 0;
+    for (int i = lane; i - lane < n; i += 64) count += __popcll(__ballot(i < n && keys[i] >= cand));
+    if (count >= want) thr = cand;
+  }
+  int above = 0;
+  for (int i = lane; i - lane < n; i += 64) above += __popcll(__ballot(i < n && keys[i] > thr));
+  int equal = want - above, at = 0;
+  for (int i = lane; i - lane < n; i += 64) {
+    const uint64_t key = i < n ? keys[i] : 0;
+    const bool eq = i < n && key == thr;
+    const uint64_t eqs = __ballot(eq), below = (uint64_t{1} << lane) - 1;
+    const bool mine = (i < n && key > thr) || (eq && static_cast<int>(__popcll(eqs & below)) < equal);
+    equal -= min(equal, static_cast<int>(__popcll(eqs)));
+    const uint64_t taken = __ballot(mine);
+    if (mine) take(at + static_cast<int>(__popcll(taken & below)), i, key);
+    at += __popcll(taken);
+  }
+}
+
+__device__ __forceinline__ double score64(const float* q, const float* m, int dim) {
+  double sum = 0.0;
+  for (int d = 0; d < dim; ++d) sum += static_cast<double>(q[d]) * static_cast<double>(m[d]);
+  return sum;
+}
+
+}  // namespace
+
+// Rows of up to kSelBlocks blocks: a workgroup takes 16 `tiles` rows (queries of
+// one key head, in token order) and scores them on fp64 MFMA, whose sums are far
+// finer than the fp32 roundings that go to LDS as order-preserving keys. LPR
+// lanes then share a row, each with up to 32 keys in registers, and find the
+// top-th largest key bit by bit, ending with the first threshold that exactly
+// `top` keys reach (some 20 steps, two instructions per key each). Where fp32
+// cannot tell the last ones apart, the row is settled with 64-bit scores.
+//
+// One wave per row with 64-bit scores summed lane by lane and a ballot per step
+// took 2.2 ms for 7,930 queries of 20 heads.
+constexpr int kSelBlocks = 960;  // a 16-row tile's keys fit 64 KB of LDS
+
+template <int DT, int DH>
+__global__ __launch_bounds__(1024) void select_rows_kernel(BlockAttnArgs p, SeqTable t, SelectPlan g) {
+  using T = typename ElemOf<DT>::T;
+  constexpr int kDims = DH / 4;  // dims per lane: kq * kDims .. + kDims
+  extern __shared__ __align__(16) uint32_t keys[];
+  __shared__ int unsettled[64];
+  __shared__ float qs[kMaxHeadDim];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int hk = blockIdx.x % p.kv_heads, wg = blockIdx.x / p.kv_heads, each = p.heads / p.kv_heads;
+  const int b = seq_of(t, t.ct, 3, wg);
+  const int q0 = table_at(t, t.cu_q, 0, b), q1 = table_at(t, t.cu_q, 0, b + 1);
+  const int b0 = table_at(t, t.cb, 2, b), nb = table_at(t, t.cb, 2, b + 1) - b0;
+  const int row0 = (wg - table_at(t, t.ct, 3, b)) * 16 * g.tiles, rows = min((q1 - q0) * each - row0, 16 * g.tiles);
+  const int want = min(p.top, nb);
+  auto token_of = [&](int row) { return q0 + (row0 + row) / each; };
+  auto head_of = [&](int row) { return hk * each + (row0 + row) % each; };
+  for (int i = threadIdx.x; i < 64; i += blockDim.x) unsettled[i] = 0;
+
+  // Scores: D = means . q^T, blocks down, queries across; lane (l % 16, kq) gives
+  // block or query l % 16 the dims of kq, one per step.
+  {
+    const int lr = lane & 15, kq = lane >> 4, d0 = kq * kDims;
+    const int row = wave % g.tiles * 16 + lr;
+    double qd[kDims];
+    const int rl = min(row, rows - 1);
+    const T* q = static_cast<const T*>(p.q) + static_cast<size_t>(token_of(rl)) * p.ldq + head_of(rl) * p.head_dim;
+#pragma unroll
+    for (int i = 0; i < kDims; ++i)
+      qd[i] = d0 + i < p.head_dim ? static_cast<double>(static_cast<float>(q[d0 + i])) : 0.0;
+    for (int bt = wave / g.tiles * 16; bt < nb; bt += waves / g.tiles * 16) {
+      const float* m =
+          p.means + (static_cast<size_t>(b0 + min(bt + lr, nb - 1)) * p.kv_heads + hk) * p.head_dim;
+      float mf[kDims];
+#pragma unroll
+      for (int i = 0; i < kDims; i += 4) {
+        const f32x4 v = d0 + i < p.head_dim ? *reinterpret_cast<const f32x4u*>(m + d0 + i) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mf[i + k] = v[k];
+      }
+      f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+      for (int i = 0; i < kDims; ++i)
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64(static_cast<double>(mf[i]), qd[i], acc, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int block = bt + 4 * r + kq;
+        keys[row * g.pitch + block] = block < nb ? score_key32(acc[r]) : 0;
+      }
+    }
+    // Keys past the last block, up to a whole number of lanes' pieces.
+    const int from = (nb + 15) / 16 * 16;
+    for (int i = from + lane / 16 + wave / g.tiles * 4; i < g.pitch; i += waves / g.tiles * 4) keys[row * g.pitch + i] = 0;
+  }
+  __syncthreads();
+
+  // Thresholds: lane gl of a row's LPR has keys gl * per .. + per.
+  const int lpr = g.lanes, gl = lane % lpr, per = ((nb + lpr - 1) / lpr + 3) & ~3;
+  const int rows_per_wave = 64 / lpr;
+  for (int u = wave * rows_per_wave; u < rows; u += waves * rows_per_wave) {
+    const int row = u + lane / lpr;
+    u32x4 k4[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (4 * i < per) {
+        const int at = gl * per + 4 * i;
+        k4[i] = at < g.pitch ? *reinterpret_cast<const u32x4*>(keys + min(row, rows - 1) * g.pitch + at)
+                             : u32x4{0, 0, 0, 0};
+      }
+    auto count_from = [&](uint32_t least) {
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (4 * i < per) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) n += k4[i][k] >= least;
+        }
+      return n;
+    };
+    auto row_sum = [&](int v) {
+      v += __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, true);  // quad_perm [1, 0, 3, 2]
+      v += __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, true);  // quad_perm [2, 3, 0, 1]
+      for (int d = 4; d < lpr; d *= 2) v += __shfl_xor(v, d);
+      return v;
+    };
+    uint32_t thr = 1;  // every block's key is at least 1
+    bool settled = want == nb;
+    if (!__all(settled)) {
+      thr = settled ? 1 : 0;
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t cand = thr | (1u << bit);
+        const int n = row_sum(count_from(cand));
+        if (!settled && n >= want) {
+          thr = cand;
+          settled = n == want;
+        }
+        if (__all(settled)) break;
+      }
+    }
+    if (row >= rows) continue;
+    int* out = p.blocks_out + (static_cast<size_t>(token_of(row)) * p.heads + head_of(row)) * p.top;
+    for (int i = want + gl; i < p.top; i += lpr) out[i] = -1;
+    if (!settled) {
+      if (gl == 0) unsettled[row] = 1;
+      continue;
+    }
+    const int mine = count_from(thr);
+    int at = mine;
+    for (int d = 1; d < lpr; d *= 2) {
+      const int v = __shfl_up(at, d);
+      at += gl >= d ? v : 0;
+    }
+    at -= mine;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (4 * i < per) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k4[i][k] >= thr) out[at++] = gl * per + 4 * i + k;
+      }
+  }
+
+  // Rows whose last blocks are equal in fp32.
+  __syncthreads();
+  for (int row = 0; row < rows; ++row) {
+    if (!unsettled[row]) continue;
+    uint64_t* keys64 = reinterpret_cast<uint64_t*>(keys);  // every row's keys are done with
+    const T* q = static_cast<const T*>(p.q) + static_cast<size_t>(token_of(row)) * p.ldq + head_of(row) * p.head_dim;
+    for (int d = threadIdx.x; d < p.head_dim; d += blockDim.x) qs[d] = static_cast<float>(q[d]);
+    __syncthreads();
+    for (int j = threadIdx.x; j < nb; j += blockDim.x)
+      keys64[j] = score_key(
+          score64(qs, p.means + (static_cast<size_t>(b0 + j) * p.kv_heads + hk) * p.head_dim, p.head_dim));
+    __syncthreads();
+    if (wave == 0) {
+      int* out = p.blocks_out + (static_cast<size_t>(token_of(row)) * p.heads + head_of(row)) * p.top;
+      take_largest(keys64, nb, want, [&](int at, int i, uint64_t) { out[at] = i; });
+    }
+    __syncthreads();
+  }
+}
+
+// Rows of any number of blocks, one wave per (query, head): 64-bit scores,
+// kSelChunk blocks at a time behind the `top` kept from the chunks before.
 constexpr int kSelChunk = 1024;
 template <int DT>
 __global__ __launch_bounds__(64) void select_blocks_kernel(BlockAttnArgs p, SeqTable t) {
@@ -148,41 +346,20 @@ __global__ __launch_bounds__(64) void select_blocks_kernel(BlockAttnArgs p, SeqT
   for (int c0 = 0; c0 < nb; c0 += kSelChunk) {
     const int nc = min(kSelChunk, nb - c0);
     for (int i = lane; i < nc; i += 64) {
-      const float* m = p.means + (static_cast<size_t>(s.b0 + c0 + i) * p.kv_heads + hk) * p.head_dim;
-      double sum = 0.0;
-      for (int d = 0; d < p.head_dim; ++d) sum += static_cast<double>(qs[d]) * static_cast<double>(m[d]);
-      keys[kept + i] = score_key(sum);
+      keys[kept + i] = score_key(
+          score64(qs, p.means + (static_cast<size_t>(s.b0 + c0 + i) * p.kv_heads + hk) * p.head_dim, p.head_dim));
       ids[kept + i] = c0 + i;
     }
     __syncthreads();
-    const int n = kept + nc, want = min(p.top, n);
-    uint64_t thr = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-      const uint64_t cand = thr | (uint64_t{1} << bit);
-      int count = 0;
-      for (int i = lane; i - lane < n; i += 64) count += __popcll(__ballot(i < n && keys[i] >= cand));
-      if (count >= want) thr = cand;
-    }
-    int above = 0;
-    for (int i = lane; i - lane < n; i += 64) above += __popcll(__ballot(i < n && keys[i] > thr));
-    int equal = want - above, at = 0;
-    for (int i = lane; i - lane < n; i += 64) {
-      const uint64_t key = i < n ? keys[i] : 0;
-      const int id = i < n ? ids[i] : 0;
-      const bool eq = i < n && key == thr;
-      const uint64_t eqs = __ballot(eq), below = (uint64_t{1} << lane) - 1;
-      const bool take = (i < n && key > thr) || (eq && static_cast<int>(__popcll(eqs & below)) < equal);
-      equal -= min(equal, static_cast<int>(__popcll(eqs)));
-      const uint64_t takes = __ballot(take);
-      __syncthreads();
-      if (take) {
-        keys[at + __popcll(takes & below)] = key;
-        ids[at + __popcll(takes & below)] = id;
-      }
-      __syncthreads();
-      at += __popcll(takes);
-    }
-    kept = want;
+    // What is kept moves to the front, never past where it is read from.
+    const int n = kept + nc;
+    kept = min(p.top, n);
+    take_largest(keys, n, kept, [&](int at, int i, uint64_t key) {
+      const int id = ids[i];
+      keys[at] = key;
+      ids[at] = id;
+    });
+    __syncthreads();
   }
   int* out = p.blocks_out + (static_cast<size_t>(row) * p.heads + head) * p.top;
   for (int i = lane; i < p.top; i += 64) out[i] = i < kept ? ids[i] : -1;
@@ -888,15 +1065,55 @@ hipError_t launch_block_means(const BlockAttnArgs& p, const SeqTable& t, int typ
   return hipGetLastError();
 }
 
-hipError_t launch_select_blocks(const BlockAttnArgs& p, const SeqTable& t, int type, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(p.rows) * p.heads;
-  if (type == kTypeF32)
-    select_blocks_kernel<kTypeF32><<<grid, 64, 0, s>>>(p, t);
-  else if (type == kTypeF16)
-    select_blocks_kernel<kTypeF16><<<grid, 64, 0, s>>>(p, t);
+namespace {
+
+template <int DT>
+hipError_t launch_select_typed(const BlockAttnArgs& p, const SeqTable& t, const SelectPlan& g, hipStream_t s) {
+  if (!g.tiles) {
+    select_blocks_kernel<DT><<<static_cast<unsigned>(p.rows) * p.heads, 64, 0, s>>>(p, t);
+    return hipGetLastError();
+  }
+  const unsigned grid = static_cast<unsigned>(g.workgroups) * p.kv_heads, block = 64 * g.waves;
+  const size_t lds = static_cast<size_t>(16) * g.tiles * g.pitch * 4;
+  if (p.head_dim <= 16)
+    select_rows_kernel<DT, 16><<<grid, block, lds, s>>>(p, t, g);
+  else if (p.head_dim <= 32)
+    select_rows_kernel<DT, 32><<<grid, block, lds, s>>>(p, t, g);
+  else if (p.head_dim <= 64)
+    select_rows_kernel<DT, 64><<<grid, block, lds, s>>>(p, t, g);
   else
-    select_blocks_kernel<kTypeBF16><<<grid, 64, 0, s>>>(p, t);
+    select_rows_kernel<DT, 128><<<grid, block, lds, s>>>(p, t, g);
   return hipGetLastError();
+}
+
+}  // namespace
+
+SelectPlan select_blocks_plan(const BlockAttnArgs& p, const int* cu_q, int batch, int max_blocks) {
+  SelectPlan g;
+  if (max_blocks > kSelBlocks) return g;
+  while (g.lanes * 32 < max_blocks) g.lanes *= 2;
+  g.pitch = (max_blocks + 63) / 64 * 64 + 4;
+  // Four tiles, one to a wave, where that leaves a workgroup for every CU and
+  // LDS for two of them on one; else one tile for all waves.
+  const size_t many = static_cast<size_t>(p.rows) * p.heads / 64;
+  g.tiles = many >= static_cast<size_t>(device_cus()) && g.pitch <= 256 ? 4 : 1;
+  g.waves = g.tiles == 4 ? 4 : std::max(4, std::min(16, (max_blocks + 15) / 16));
+  size_t n = 0;
+  for (int b = 0; b < batch; ++b) n += select_workgroups(p, g, cu_q[b + 1] - cu_q[b]);
+  g.workgroups = static_cast<int>(n);  // at most one per (query, head)
+  return g;
+}
+
+int select_workgroups(const BlockAttnArgs& p, const SelectPlan& g, int queries) {
+  const size_t rows = static_cast<size_t>(queries) * (p.heads / p.kv_heads);
+  return g.tiles ? static_cast<int>((rows + 16 * g.tiles - 1) / (16 * g.tiles)) : 0;
+}
+
+hipError_t launch_select_blocks(const BlockAttnArgs& p, const SeqTable& t, const SelectPlan& g, int type,
+                                hipStream_t s) {
+  if (type == kTypeF32) return launch_select_typed<kTypeF32>(p, t, g, s);
+  if (type == kTypeF16) return launch_select_typed<kTypeF16>(p, t, g, s);
+  return launch_select_typed<kTypeBF16>(p, t, g, s);
 }
 
 namespace {

@@ -1010,29 +1010,32 @@ int blocks_of(int n, int block_size) { return n > 0 ? (n - 1) / block_size + 1 :
 // Fills the table of a batch of the block attention ops: in the kernel's
 // arguments up to kInlineSeqs sequences, else copied to op scratch behind
 // `reserve` bytes (through the pinned staging up to its size). cu_q may be null
-// (block means). Returns with *reserved pointing at the scratch when reserve > 0.
-int stage_sequences(esm_gfx950_ctx* ctx, const int* cu_q, const int* cu_k, int batch, int block_size, size_t reserve,
-                    SeqTable* t, void** reserved) {
+// (block means), select where no selection follows. Returns with *reserved
+// pointing at the scratch when reserve > 0.
+int stage_sequences(esm_gfx950_ctx* ctx, const int* cu_q, const int* cu_k, int batch, const BlockAttnArgs& p,
+                    const SelectPlan* select, size_t reserve, SeqTable* t, void** reserved) {
   t->batch = batch;
   const size_t n = static_cast<size_t>(batch) + 1;
   std::vector<int> host;
-  int *hq = t->cu_q, *hk = t->cu_k, *hb = t->cb;
+  int *hq = t->cu_q, *hk = t->cu_k, *hb = t->cb, *ht = t->ct;
   if (batch > kInlineSeqs) {
-    host.resize(3 * n);
+    host.resize(4 * n);
     hq = host.data();
     hk = hq + n;
     hb = hk + n;
+    ht = hb + n;
   }
   for (size_t i = 0; i < n; ++i) {
     hq[i] = cu_q ? cu_q[i] : 0;
     hk[i] = cu_k[i];
-    hb[i] = i == 0 ? 0 : hb[i - 1] + blocks_of(cu_k[i] - cu_k[i - 1], block_size);
+    hb[i] = i == 0 ? 0 : hb[i - 1] + blocks_of(cu_k[i] - cu_k[i - 1], p.block_size);
+    ht[i] = i == 0 || !select ? 0 : ht[i - 1] + select_workgroups(p, *select, cu_q[i] - cu_q[i - 1]);
   }
   if (batch <= kInlineSeqs) {
     if (reserve) ESM_TRY(ctx->get_scratch(reserve, reserved));
     return ESM_GFX950_OK;
   }
-  const size_t bytes = 3 * n * 4, at = align_up(reserve, 256);
+  const size_t bytes = 4 * n * 4, at = align_up(reserve, 256);
   void* s = nullptr;
   ESM_TRY(ctx->get_scratch(at + bytes, &s));
   *reserved = s;
@@ -1102,9 +1105,6 @@ extern "C" int esm_gfx950_key_block_means(esm_gfx950_ctx* ctx, const void* k, in
               "key_block_means: means shares memory with k");
   DeviceScope on(ctx);
   try {
-    SeqTable t;
-    void* unused = nullptr;
-    ESM_TRY(stage_sequences(ctx, nullptr, cu_k, batch_size, block_size, 0, &t, &unused));
     BlockAttnArgs p;
     p.k = k;
     p.ldkv = ldk;
@@ -1113,6 +1113,9 @@ extern "C" int esm_gfx950_key_block_means(esm_gfx950_ctx* ctx, const void* k, in
     p.block_size = block_size;
     p.num_blocks = static_cast<int>(blocks);
     p.means_out = means;
+    SeqTable t;
+    void* unused = nullptr;
+    ESM_TRY(stage_sequences(ctx, nullptr, cu_k, batch_size, p, nullptr, 0, &t, &unused));
     ESM_HIP(ctx, launch_block_means(p, t, dtype, ctx->stream));
   } catch (const std::exception& e) {
     return ctx->fail(ESM_GFX950_INTERNAL, std::string("key_block_means: ") + e.what());
@@ -1144,9 +1147,6 @@ extern "C" int esm_gfx950_attention_select_blocks(esm_gfx950_ctx* ctx, const voi
               "attention_select_blocks: blocks shares memory with an input");
   DeviceScope on(ctx);
   try {
-    SeqTable t;
-    void* unused = nullptr;
-    ESM_TRY(stage_sequences(ctx, cu_q, cu_k, batch_size, block_size, 0, &t, &unused));
     BlockAttnArgs p;
     p.q = q;
     p.ldq = ldq;
@@ -1159,7 +1159,14 @@ extern "C" int esm_gfx950_attention_select_blocks(esm_gfx950_ctx* ctx, const voi
     p.num_blocks = static_cast<int>(n_blocks);
     p.means = means;
     p.blocks_out = blocks;
-    ESM_HIP(ctx, launch_select_blocks(p, t, dtype, ctx->stream));
+    int max_blocks = 0;
+    for (int b = 0; b < batch_size; ++b)
+      if (cu_q[b + 1] > cu_q[b]) max_blocks = std::max(max_blocks, blocks_of(cu_k[b + 1] - cu_k[b], block_size));
+    const SelectPlan plan = select_blocks_plan(p, cu_q, batch_size, max_blocks);
+    SeqTable t;
+    void* unused = nullptr;
+    ESM_TRY(stage_sequences(ctx, cu_q, cu_k, batch_size, p, &plan, 0, &t, &unused));
+    ESM_HIP(ctx, launch_select_blocks(p, t, plan, dtype, ctx->stream));
   } catch (const std::exception& e) {
     return ctx->fail(ESM_GFX950_INTERNAL, std::string("attention_select_blocks: ") + e.what());
   }
@@ -1211,7 +1218,7 @@ extern "C" int esm_gfx950_attention_blocks(esm_gfx950_ctx* ctx, const void* q, i
     const BlockAttnPlan plan = attention_blocks_plan(p);
     SeqTable t;
     void* scratch = nullptr;
-    ESM_TRY(stage_sequences(ctx, cu_q, cu_k, batch_size, block_size, plan.scratch_bytes, &t, &scratch));
+    ESM_TRY(stage_sequences(ctx, cu_q, cu_k, batch_size, p, nullptr, plan.scratch_bytes, &t, &scratch));
     ESM_HIP(ctx, launch_attention_blocks(p, t, plan, scratch, dtype, ctx->stream));
   } catch (const std::exception& e) {
     return ctx->fail(ESM_GFX950_INTERNAL, std::string("attention_blocks: ") + e.what());

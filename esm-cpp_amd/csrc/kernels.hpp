@@ -367,10 +367,11 @@ void linear_i4_layout(const uint8_t* packed, const float* scales, int N, int K, 
 constexpr int kInlineSeqs = 64;
 struct SeqTable {
   int batch = 0;
-  const int* dev = nullptr;  // cu_q, cu_k, cb one after the other, batch + 1 each
+  const int* dev = nullptr;  // cu_q, cu_k, cb, ct one after the other, batch + 1 each
   int cu_q[kInlineSeqs + 1];
   int cu_k[kInlineSeqs + 1];
   int cb[kInlineSeqs + 1];
+  int ct[kInlineSeqs + 1];  // first workgroup (of a key head) of the selection
 };
 struct BlockAttnArgs {
   const void* q = nullptr;  // [rows, heads, head_dim], row stride ldq
@@ -389,7 +390,21 @@ struct BlockAttnArgs {
 };
 constexpr int kMaxHeadDim = 128, kMaxTop = 256;
 hipError_t launch_block_means(const BlockAttnArgs& p, const SeqTable& t, int type, hipStream_t s);
-hipError_t launch_select_blocks(const BlockAttnArgs& p, const SeqTable& t, int type, hipStream_t s);
+// How the selection runs: workgroups of 16 `tiles` rows (queries x the heads of
+// a key head) of one sequence, the table's ct their running count by sequence;
+// tiles 0: one wave per (query, head).
+struct SelectPlan {
+  int tiles = 0;
+  int lanes = 4;       // lanes that share a row's threshold search
+  int pitch = 0;       // keys per row in LDS
+  int waves = 4;
+  int workgroups = 0;  // per key head
+};
+// max_blocks: the most blocks of a sequence with queries (host cu_q).
+SelectPlan select_blocks_plan(const BlockAttnArgs& p, const int* cu_q, int batch, int max_blocks);
+int select_workgroups(const BlockAttnArgs& p, const SelectPlan& g, int queries);
+hipError_t launch_select_blocks(const BlockAttnArgs& p, const SeqTable& t, const SelectPlan& g, int type,
+                                hipStream_t s);
 // How attention_blocks runs: row by row, or block by block (grouped) for
 // `tokens` tokens and `kv_heads` key heads at a time.
 struct BlockAttnPlan {
