@@ -129,11 +129,30 @@ namespace {
 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
-// Order-preserving 32-bit key of a score's fp32 rounding, never 0.
-__device__ __forceinline__ uint32_t score_key32(double s) {
-  if (s != s) s = -INFINITY;
-  const uint32_t u = __float_as_uint(static_cast<float>(s + 0.0) + 0.0f);
+// Order-preserving 32-bit key of an fp32 score, never 0.
+__device__ __forceinline__ uint32_t score_key32(float s) {
+  const uint32_t u = __float_as_uint(s + 0.0f);
   return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+// f over the lpr (4 .. 64) lanes that share a row, without a trip through LDS:
+// quad permutations, then mirrors of 8 and 16 lanes (each half is uniform by
+// then), then lane swaps.
+template <class F>
+__device__ __forceinline__ uint32_t row_reduce(uint32_t v, int lpr, F f) {
+  v = f(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, true)));  // quad_perm [1, 0, 3, 2]
+  v = f(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, true)));  // quad_perm [2, 3, 0, 1]
+  if (lpr > 4) v = f(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true)));  // row_half_mirror
+  if (lpr > 8) v = f(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true)));  // row_mirror
+  if (lpr > 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = f(r[0], r[1]);
+  }
+  if (lpr > 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = f(r[0], r[1]);
+  }
+  return v;
 }
 
 // One wave: of the n 64-bit keys, the `want` largest (ties to the lowest index),
@@ -174,10 +193,11 @@ __device__ __forceinline__ double score64(const float* q, const float* m, int di
 
 // Rows of up to kSelBlocks blocks: a workgroup takes 16 `tiles` rows (queries of
 // one key head, in token order) and scores them on fp64 MFMA, whose sums are far
-// finer than the fp32 roundings that go to LDS as order-preserving keys. LPR
-// lanes then share a row, each with up to 32 keys in registers, and find the
-// top-th largest key bit by bit, ending with the first threshold that exactly
-// `top` keys reach (some 20 steps, two instructions per key each). Where fp32
+// finer than the fp32 roundings that go to LDS. LPR lanes then share a row, each
+// with up to 32 scores in registers, as integers spread evenly over the row's
+// range, and find the top-th largest bit by bit, ending with the first threshold
+// that exactly `top` of them reach (about as many steps as the row's range is
+// powers of two of the gap there, two instructions per score each). Where that
 // cannot tell the last ones apart, the row is settled with 64-bit scores.
 //
 // One wave per row with 64-bit scores summed lane by lane and a ballot per step
@@ -188,7 +208,7 @@ template <int DT, int DH>
 __global__ __launch_bounds__(1024) void select_rows_kernel(BlockAttnArgs p, SeqTable t, SelectPlan g) {
   using T = typename ElemOf<DT>::T;
   constexpr int kDims = DH / 4;  // dims per lane: kq * kDims .. + kDims
-  extern __shared__ __align__(16) uint32_t keys[];
+  extern __shared__ __align__(16) float scores[];
   __shared__ int unsettled[64];
   __shared__ float qs[kMaxHeadDim];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
@@ -210,76 +230,114 @@ __global__ __launch_bounds__(1024) void select_rows_kernel(BlockAttnArgs p, SeqT
     double qd[kDims];
     const int rl = min(row, rows - 1);
     const T* q = static_cast<const T*>(p.q) + static_cast<size_t>(token_of(rl)) * p.ldq + head_of(rl) * p.head_dim;
+    // Loads without conditions (each of which would be waited for on its own):
+    // dims past the head read its last four, and count as zero.
+    const int last = p.head_dim - 4;
+    T qx[kDims];
 #pragma unroll
-    for (int i = 0; i < kDims; ++i)
-      qd[i] = d0 + i < p.head_dim ? static_cast<double>(static_cast<float>(q[d0 + i])) : 0.0;
-    for (int bt = wave / g.tiles * 16; bt < nb; bt += waves / g.tiles * 16) {
+    for (int i = 0; i < kDims; i += 4) {
+      const T* at = q + min(d0 + i, last);
+      if constexpr (DT == kTypeF32) {
+        const f32x4 v = *reinterpret_cast<const f32x4u*>(at);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) qx[i + k] = v[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) qx[i + k] = at[k];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kDims; ++i) qd[i] = d0 + i < p.head_dim ? static_cast<double>(static_cast<float>(qx[i])) : 0.0;
+    const int step = waves / g.tiles * 16;
+    float mf[kDims], next[kDims];
+    auto load = [&](int bt, float (&to)[kDims]) {
       const float* m =
           p.means + (static_cast<size_t>(b0 + min(bt + lr, nb - 1)) * p.kv_heads + hk) * p.head_dim;
-      float mf[kDims];
 #pragma unroll
       for (int i = 0; i < kDims; i += 4) {
-        const f32x4 v = d0 + i < p.head_dim ? *reinterpret_cast<const f32x4u*>(m + d0 + i) : f32x4{0.f, 0.f, 0.f, 0.f};
+        const f32x4 v = *reinterpret_cast<const f32x4u*>(m + min(d0 + i, last));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mf[i + k] = v[k];
+        for (int k = 0; k < 4; ++k) to[i + k] = d0 + i < p.head_dim ? v[k] : 0.0f;
       }
+    };
+    int bt = wave / g.tiles * 16;
+    if (bt < nb) load(bt, next);
+    for (; bt < nb; bt += step) {
+#pragma unroll
+      for (int i = 0; i < kDims; ++i) mf[i] = next[i];
+      if (bt + step < nb) load(bt + step, next);
       f64x4 acc = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
       for (int i = 0; i < kDims; ++i)
         acc = __builtin_amdgcn_mfma_f64_16x16x4f64(static_cast<double>(mf[i]), qd[i], acc, 0, 0, 0);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int block = bt + 4 * r + kq;
-        keys[row * g.pitch + block] = block < nb ? score_key32(acc[r]) : 0;
+        const float s = static_cast<float>(acc[r]);
+        scores[row * g.pitch + bt + 4 * r + kq] = s != s ? -INFINITY : s;
       }
     }
-    // Keys past the last block, up to a whole number of lanes' pieces.
-    const int from = (nb + 15) / 16 * 16;
-    for (int i = from + lane / 16 + wave / g.tiles * 4; i < g.pitch; i += waves / g.tiles * 4) keys[row * g.pitch + i] = 0;
   }
   __syncthreads();
 
-  // Thresholds: lane gl of a row's LPR has keys gl * per .. + per.
+  // Thresholds: lane gl of a row's LPR has scores gl * per .. + per.
   const int lpr = g.lanes, gl = lane % lpr, per = ((nb + lpr - 1) / lpr + 3) & ~3;
   const int rows_per_wave = 64 / lpr;
   for (int u = wave * rows_per_wave; u < rows; u += waves * rows_per_wave) {
     const int row = u + lane / lpr;
-    u32x4 k4[8];
+    // A lane's scores, the number of which is uniform: four at a time.
+    f32x4 s4[8];
+    float most = -INFINITY, least = INFINITY;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (4 * i < per) {
         const int at = gl * per + 4 * i;
-        k4[i] = at < g.pitch ? *reinterpret_cast<const u32x4*>(keys + min(row, rows - 1) * g.pitch + at)
-                             : u32x4{0, 0, 0, 0};
+        if (at < g.pitch) s4[i] = *reinterpret_cast<const f32x4*>(scores + min(row, rows - 1) * g.pitch + at);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (at + k < nb) {
+            most = fmaxf(most, s4[i][k]);
+            least = fminf(least, s4[i][k]);
+          }
       }
-    auto count_from = [&](uint32_t least) {
+    auto as_max = [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); };
+    auto as_min = [](uint32_t a, uint32_t b) { return __float_as_uint(fminf(__uint_as_float(a), __uint_as_float(b))); };
+    auto add = [](uint32_t a, uint32_t b) { return a + b; };
+    most = __uint_as_float(row_reduce(__float_as_uint(most), lpr, as_max));
+    least = __uint_as_float(row_reduce(__float_as_uint(least), lpr, as_min));
+    // Keys 1 .. 2^30 over the row's range where that is finite, else the ordered
+    // bits; 0 past the last block. Both keep the order of the scores.
+    const float range = most - least;
+    const bool even = range > 1e-30f && range < INFINITY;
+    const float unit = even ? 1073741696.0f / range : 0.0f;
+    uint32_t k4[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (4 * i < per) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t key =
+              even ? 1u + static_cast<uint32_t>((s4[i][k] - least) * unit) : score_key32(s4[i][k]);
+          k4[i][k] = gl * per + 4 * i + k < nb ? key : 0;
+        }
+      }
+    auto count_from = [&](uint32_t from) {
       int n = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (4 * i < per) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) n += k4[i][k] >= least;
+          for (int k = 0; k < 4; ++k) n += k4[i][k] >= from;
         }
       return n;
     };
-    auto row_sum = [&](int v) {
-      v += __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, true);  // quad_perm [1, 0, 3, 2]
-      v += __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, true);  // quad_perm [2, 3, 0, 1]
-      for (int d = 4; d < lpr; d *= 2) v += __shfl_xor(v, d);
-      return v;
-    };
-    uint32_t thr = 1;  // every block's key is at least 1
+    uint32_t thr = want == nb ? 1 : 0;  // every block's key is at least 1
     bool settled = want == nb;
-    if (!__all(settled)) {
-      thr = settled ? 1 : 0;
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t cand = thr | (1u << bit);
-        const int n = row_sum(count_from(cand));
-        if (!settled && n >= want) {
-          thr = cand;
-          settled = n == want;
-        }
-        if (__all(settled)) break;
+    for (int bit = __all(even) ? 30 : 31; bit >= 0 && !__all(settled); --bit) {
+      const uint32_t cand = thr | (1u << bit);
+      const int n = static_cast<int>(row_reduce(count_from(cand), lpr, add));
+      if (!settled && n >= want) {
+        thr = cand;
+        settled = n == want;
       }
     }
     if (row >= rows) continue;
@@ -305,11 +363,11 @@ __global__ __launch_bounds__(1024) void select_rows_kernel(BlockAttnArgs p, SeqT
       }
   }
 
-  // Rows whose last blocks are equal in fp32.
+  // Rows whose last blocks are equal so far.
   __syncthreads();
   for (int row = 0; row < rows; ++row) {
     if (!unsettled[row]) continue;
-    uint64_t* keys64 = reinterpret_cast<uint64_t*>(keys);  // every row's keys are done with
+    uint64_t* keys64 = reinterpret_cast<uint64_t*>(scores);  // every row's scores are done with
     const T* q = static_cast<const T*>(p.q) + static_cast<size_t>(token_of(row)) * p.ldq + head_of(row) * p.head_dim;
     for (int d = threadIdx.x; d < p.head_dim; d += blockDim.x) qs[d] = static_cast<float>(q[d]);
     __syncthreads();
@@ -1092,7 +1150,7 @@ SelectPlan select_blocks_plan(const BlockAttnArgs& p, const int* cu_q, int batch
   SelectPlan g;
   if (max_blocks > kSelBlocks) return g;
   while (g.lanes * 32 < max_blocks) g.lanes *= 2;
-  g.pitch = (max_blocks + 63) / 64 * 64 + 4;
+  g.pitch = (max_blocks + 15) / 16 * 16 + 4;  // 16 rows of 4 scores fall on distinct banks
   // Four tiles, one to a wave, where that leaves a workgroup for every CU and
   // LDS for two of them on one; else one tile for all waves.
   const size_t many = static_cast<size_t>(p.rows) * p.heads / 64;

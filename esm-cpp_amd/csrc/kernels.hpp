@@ -396,7 +396,7 @@ hipError_t launch_block_means(const BlockAttnArgs& p, const SeqTable& t, int typ
 struct SelectPlan {
   int tiles = 0;
   int lanes = 4;       // lanes that share a row's threshold search
-  int pitch = 0;       // keys per row in LDS
+  int pitch = 0;       // scores per row in LDS
   int waves = 4;
   int workgroups = 0;  // per key head
 };
