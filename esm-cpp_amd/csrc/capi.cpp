@@ -1072,7 +1072,8 @@ int check_block_shape(esm_gfx950_ctx* ctx, const char* op, int heads, int kv_hea
   ESM_REQUIRE(ctx, heads > 0 && kv_heads > 0 && heads % kv_heads == 0, at + "num_kv_heads must divide num_heads");
   ESM_REQUIRE(ctx, head_dim > 0 && head_dim <= kMaxHeadDim && head_dim % 8 == 0,
               at + "head_dim must be a multiple of 8, at most 128");
-  ESM_REQUIRE(ctx, heads <= 0x7fffffff / kMaxHeadDim, at + "too many heads");
+  // Rows of at most 2^22 elements (kMaxRowStride) need no more heads than that.
+  ESM_REQUIRE(ctx, heads <= kMaxRowStride, at + "too many heads");
   ESM_REQUIRE(ctx, block_size_ok(block_size), at + "block_size must be a multiple of 16, 16..1024");
   return ESM_GFX950_OK;
 }
@@ -1113,6 +1114,7 @@ extern "C" int esm_gfx950_key_block_means(esm_gfx950_ctx* ctx, const void* k, in
     p.block_size = block_size;
     p.num_blocks = static_cast<int>(blocks);
     p.means_out = means;
+    p.vec_kv = aligned(k, 16) && static_cast<size_t>(ldk) * size % 16 == 0;
     SeqTable t;
     void* unused = nullptr;
     ESM_TRY(stage_sequences(ctx, nullptr, cu_k, batch_size, p, nullptr, 0, &t, &unused));
