@@ -995,7 +995,10 @@ extern "C" int esm_gfx950_linear_i4(esm_gfx950_ctx* ctx, const void* A, int lda,
   p.groups = W->groups;
   p.tiles_k = W->tiles_k;
   p.vec_a = aligned(A, 16) && static_cast<size_t>(lda) * size % 16 == 0;
-  ESM_HIP(ctx, launch_linear_i4(p, dtype, ctx->stream));
+  const LinearI4Plan plan = linear_i4_plan(p, dtype);
+  void* scratch = nullptr;
+  if (plan.scratch_bytes) ESM_TRY(ctx->get_scratch(plan.scratch_bytes, &scratch));
+  ESM_HIP(ctx, launch_linear_i4(p, plan, scratch, dtype, ctx->stream));
   return ESM_GFX950_OK;
 }
 

@@ -355,7 +355,15 @@ struct LinearI4Args {
   int tiles_k = 0;  // ceil(K / 128)
   bool vec_a = false;  // A's rows start at 16-byte addresses
 };
-hipError_t launch_linear_i4(const LinearI4Args& p, int type, hipStream_t s);
+// How linear_i4 runs: 16 row_tiles rows at a time with the activations split in
+// the kernel, or as a GEMM on activations split into scratch beforehand.
+struct LinearI4Plan {
+  bool gemm = false;
+  int row_tiles = 1;
+  size_t scratch_bytes = 0;
+};
+LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type);
+hipError_t launch_linear_i4(const LinearI4Args& p, const LinearI4Plan& plan, void* scratch, int type, hipStream_t s);
 // The device layout (host): w of 256 dwords per 16 x 128 tile, zero codes past N
 // and K; s [tiles_n, groups, 16], zeros past N.
 void linear_i4_layout(const uint8_t* packed, const float* scales, int N, int K, int group, uint32_t* w, float* s);

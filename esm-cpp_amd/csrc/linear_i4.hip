@@ -208,12 +208,210 @@ __global__ __launch_bounds__(512) void linear_i4_rows_kernel(LinearI4Args p) {
   }
 }
 
+// ------------------------------------------------------------- many rows
+// Activations as the matrix cores take them, written once for every column tile:
+// fp16 planes [planes][M][ldp] (hi, and lo for fp32), zeros past K, a row scaled
+// by the power of two that brings its largest to [2^14, 2^15) (fp16 rows are
+// taken as they are), the power's inverse in inv. One workgroup per row.
+template <int DT>
+__global__ __launch_bounds__(256) void linear_i4_split_kernel(LinearI4Args p, uint16_t* planes, float* inv, int ldp) {
+  using T = typename Elem<DT>::T;
+  __shared__ float part[4];
+  const int m = blockIdx.x;
+  const T* row = static_cast<const T*>(p.A) + static_cast<size_t>(m) * p.lda;
+  uint16_t* hi = planes + static_cast<size_t>(m) * ldp;
+  uint16_t* lo = hi + static_cast<size_t>(p.M) * ldp;
+  float mul = 1.0f;
+  if constexpr (DT != kTypeF16) {
+    float amax = 0.0f;
+    for (int k = threadIdx.x * 8; k < p.K; k += 2048) {
+      T x[8];
+      load8<T>(row, k, p.K, p.vec_a, x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = fabsf(static_cast<float>(x[i]));
+        amax = fmaxf(amax, v < INFINITY ? v : 0.0f);
+      }
+    }
+    amax = wave_max(amax);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = amax;
+    __syncthreads();
+    const int e = row_exponent(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
+    mul = __builtin_amdgcn_ldexpf(1.0f, e);
+    if (threadIdx.x == 0) inv[m] = __builtin_amdgcn_ldexpf(1.0f, -e);
+  } else {
+    if (threadIdx.x == 0) inv[m] = 1.0f;
+  }
+  for (int k = threadIdx.x * 8; k < ldp; k += 2048) {
+    T x[8];
+    load8<T>(row, k, p.K, p.vec_a, x);
+    f16x8 h, l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float v = static_cast<float>(x[i]) * mul;
+      h[i] = static_cast<_Float16>(v);
+      l[i] = static_cast<_Float16>(fabsf(v) < INFINITY ? v - static_cast<float>(h[i]) : 0.0f);
+    }
+    *reinterpret_cast<f16x8*>(hi + k) = h;
+    if constexpr (Elem<DT>::kPlanes == 2) *reinterpret_cast<f16x8*>(lo + k) = l;
+  }
+}
+
+// 128 x 128 outputs per workgroup, 64 x 64 per wave on v_mfma_f32_32x32x16_f16:
+// activations through LDS by direct loads, 64 inputs a stage, two stages; codes
+// straight from global memory into the operand registers, the next 128 inputs'
+// on their way. D has outputs across lanes: a group's scale is one register per
+// 32 columns.
+constexpr int kGemmM = 128, kGemmN = 128, kGemmK = 64;
+template <int DT, int GJ>  // GJ: 32-input steps of a group within 128 inputs
+__global__ __launch_bounds__(256) void linear_i4_gemm_kernel(LinearI4Args p, const uint16_t* planes, const float* inv,
+                                                             int ldp) {
+  using T = typename Elem<DT>::T;
+  constexpr int PL = Elem<DT>::kPlanes;
+  constexpr int kPlaneBytes = kGemmM * kGemmK * 2;
+  typedef float f32x16 __attribute__((ext_vector_type(16)));
+  __shared__ __align__(1024) uint8_t stage[2][PL * kPlaneBytes];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int ln = lane & 31, half = lane >> 5;
+  int m0, n0;
+  tile_origin_of(blockIdx.x, p.M, p.N, kGemmM, kGemmN, &m0, &n0);
+  const int wm = wave >> 1, wn = wave & 1;
+
+  // Direct loads: one instruction brings 8 rows of 64 inputs (1 KB); wave w loads
+  // rows 32 w .. + 32. The 16-byte piece c of row r lies at c ^ (r % 8), so that
+  // 32 rows' pieces fall on distinct banks.
+  const uint32_t lds0 = lds_byte_addr(&stage[0][0]);
+  uint32_t off[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = wave * 32 + i * 8 + (lane >> 3), c = (lane & 7) ^ (lane >> 3);
+    off[i] = static_cast<uint32_t>(min(r, p.M - 1 - m0)) * static_cast<uint32_t>(ldp * 2) + c * 16;
+  }
+  const size_t plane_elems = static_cast<size_t>(p.M) * ldp;
+  auto load_stage = [&](int k0, int buf) {
+#pragma unroll
+    for (int pl = 0; pl < PL; ++pl) {
+      const uint16_t* base = planes + pl * plane_elems + static_cast<size_t>(m0) * ldp + k0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        lds_dma16(base, off[i], lds0 + buf * (PL * kPlaneBytes) + pl * kPlaneBytes + (wave * 32 + i * 8) * 128);
+    }
+  };
+
+  // Codes: for 16 inputs s of 128, lane (n, half) takes dword s / 2 of storage lane
+  // n % 16 + 16 (2 (s % 2) + half).
+  const int tiles_n = (p.N + kTileN - 1) / kTileN;
+  const u32x4* wp[2];
+  const float* sp[2];
+#pragma unroll
+  for (int nt = 0; nt < 2; ++nt) {
+    const int tn = min((n0 + wn * 64 + nt * 32) / kTileN + (ln >> 4), tiles_n - 1);
+    wp[nt] = reinterpret_cast<const u32x4*>(p.W) + static_cast<size_t>(tn) * p.tiles_k * 64 + (ln & 15) + 16 * half;
+    sp[nt] = p.scales + static_cast<size_t>(tn) * p.groups * kTileN + (ln & 15);
+  }
+  u32x4 w[2][2], wnext[2][2];
+  float s[2][4 / GJ], snext[2][4 / GJ];
+  auto load_codes = [&](int kt, u32x4 (&to)[2][2], float (&st)[2][4 / GJ]) {
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      to[nt][0] = wp[nt][static_cast<size_t>(kt) * 64];
+      to[nt][1] = wp[nt][static_cast<size_t>(kt) * 64 + 32];
+#pragma unroll
+      for (int g = 0; g < 4 / GJ; ++g)
+        st[nt][g] = sp[nt][static_cast<size_t>(min((kt * kTileK + g * 32 * GJ) / p.group, p.groups - 1)) * kTileN];
+    }
+  };
+
+  f32x16 total[2][2], acc[2][2];
+#pragma unroll
+  for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) total[mt][nt][i] = acc[mt][nt][i] = 0.0f;
+
+  load_stage(0, 0);
+  load_codes(0, wnext, snext);
+  for (int kt = 0; kt < p.tiles_k; ++kt) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // 64 inputs each
+      // This stage has landed for every wave, and every wave is done with the other.
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (h == 0) {
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          w[nt][0] = wnext[nt][0];
+          w[nt][1] = wnext[nt][1];
+#pragma unroll
+          for (int g = 0; g < 4 / GJ; ++g) s[nt][g] = snext[nt][g];
+        }
+        load_stage(kt * kTileK + kGemmK, 1);
+      } else if (kt + 1 < p.tiles_k) {
+        load_stage((kt + 1) * kTileK, 0);
+        load_codes(kt + 1, wnext, snext);
+      }
+      const uint8_t* at = stage[h];
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        const int step = h * 4 + st;  // of the 128 inputs' eight
+        f16x8 wf[2];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) wf[nt] = unpack_codes(w[nt][step & 1][step >> 1]);
+        const bool first = step % (2 * GJ) == 0;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          const int r = wm * 64 + mt * 32 + ln;
+          const uint8_t* a = at + r * 128 + (((2 * st + half) ^ (r & 7)) << 4);
+          const f16x8 ah = *reinterpret_cast<const f16x8*>(a);
+          f16x8 al;
+          if constexpr (PL == 2) al = *reinterpret_cast<const f16x8*>(a + kPlaneBytes);
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+            if (first) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) acc[mt][nt][i] = 0.0f;
+            }
+            acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, wf[nt], acc[mt][nt], 0, 0, 0);
+            if constexpr (PL == 2) acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, wf[nt], acc[mt][nt], 0, 0, 0);
+          }
+        }
+        if (step % (2 * GJ) == 2 * GJ - 1) {
+          const int g = step / (2 * GJ);
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                total[mt][nt][i] = __builtin_fmaf(acc[mt][nt][i], s[nt][g], total[mt][nt][i]);
+        }
+      }
+    }
+  }
+
+#pragma unroll
+  for (int nt = 0; nt < 2; ++nt) {
+    const int n = n0 + wn * 64 + nt * 32 + ln;
+    const float bias = p.bias && n < p.N ? p.bias[n] : 0.0f;
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int m = m0 + wm * 64 + mt * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
+        if (m < p.M && n < p.N)
+          static_cast<T*>(p.C)[static_cast<size_t>(m) * p.ldc + n] =
+              static_cast<T>(__builtin_fmaf(total[mt][nt][i], inv[m], bias));
+      }
+  }
+}
+
 namespace {
 
 template <int DT, int MT, int NT>
 hipError_t launch_rows(const LinearI4Args& p, hipStream_t s) {
-  const int waves = std::min(8, p.tiles_k);
-  const unsigned grid = static_cast<unsigned>((p.N + 16 * NT - 1) / (16 * NT)) * ((p.M + 16 * MT - 1) / (16 * MT));
+  const int waves = std::min(NT * MT >= 16 ? 4 : 8, p.tiles_k);
+  const unsigned grid =
+      static_cast<unsigned>((p.N + 16 * NT - 1) / (16 * NT)) * ((p.M + 16 * MT - 1) / (16 * MT));
   const size_t lds = static_cast<size_t>(waves) * NT * MT * 1024;
   const dim3 block(64 * waves);
   if (p.group == 32)
@@ -226,16 +424,47 @@ hipError_t launch_rows(const LinearI4Args& p, hipStream_t s) {
 }
 
 template <int DT>
-hipError_t launch_typed(const LinearI4Args& p, hipStream_t s) {
-  return launch_rows<DT, 1, 1>(p, s);
+hipError_t launch_gemm(const LinearI4Args& p, void* scratch, hipStream_t s) {
+  const int ldp = p.tiles_k * kTileK;
+  auto* planes = static_cast<uint16_t*>(scratch);
+  auto* inv = reinterpret_cast<float*>(planes + static_cast<size_t>(Elem<DT>::kPlanes) * p.M * ldp);
+  linear_i4_split_kernel<DT><<<p.M, 256, 0, s>>>(p, planes, inv, ldp);
+  const unsigned grid =
+      static_cast<unsigned>((p.M + kGemmM - 1) / kGemmM) * static_cast<unsigned>((p.N + kGemmN - 1) / kGemmN);
+  if (p.group == 32)
+    linear_i4_gemm_kernel<DT, 1><<<grid, 256, 0, s>>>(p, planes, inv, ldp);
+  else if (p.group == 64)
+    linear_i4_gemm_kernel<DT, 2><<<grid, 256, 0, s>>>(p, planes, inv, ldp);
+  else
+    linear_i4_gemm_kernel<DT, 4><<<grid, 256, 0, s>>>(p, planes, inv, ldp);
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_typed(const LinearI4Args& p, const LinearI4Plan& plan, void* scratch, hipStream_t s) {
+  if (plan.gemm) return launch_gemm<DT>(p, scratch, s);
+  if (plan.row_tiles == 1) return launch_rows<DT, 1, 1>(p, s);
+  if (plan.row_tiles == 2) return launch_rows<DT, 2, 2>(p, s);
+  return launch_rows<DT, 4, 4>(p, s);
 }
 
 }  // namespace
 
-hipError_t launch_linear_i4(const LinearI4Args& p, int type, hipStream_t s) {
-  if (type == kTypeF32) return launch_typed<kTypeF32>(p, s);
-  if (type == kTypeF16) return launch_typed<kTypeF16>(p, s);
-  return launch_typed<kTypeBF16>(p, s);
+LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type) {
+  LinearI4Plan plan;
+  const int ldp = p.tiles_k * kTileK;
+  // A tile's 128 rows are 32-bit offsets apart.
+  plan.gemm = p.M > 256 && ldp < (1 << 23);
+  plan.row_tiles = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
+  if (plan.gemm)
+    plan.scratch_bytes = static_cast<size_t>(p.M) * (static_cast<size_t>(ldp) * (type == kTypeF32 ? 4 : 2) + 4);
+  return plan;
+}
+
+hipError_t launch_linear_i4(const LinearI4Args& p, const LinearI4Plan& plan, void* scratch, int type, hipStream_t s) {
+  if (type == kTypeF32) return launch_typed<kTypeF32>(p, plan, scratch, s);
+  if (type == kTypeF16) return launch_typed<kTypeF16>(p, plan, scratch, s);
+  return launch_typed<kTypeBF16>(p, plan, scratch, s);
 }
 
 void linear_i4_layout(const uint8_t* packed, const float* scales, int N, int K, int group, uint32_t* w, float* s) {
