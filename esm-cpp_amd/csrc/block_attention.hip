@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256) void block_means_kernel(BlockAttnArgs p, SeqTa
   using T = typename ElemOf<DT>::T;
   constexpr int E = 16 / sizeof(T);
   __shared__ double sums[3][E][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int j = blockIdx.x;
   const Seq s = seq_at(t, seq_of(t, t.cb, 2, j));
   const int t0 = s.k0 + (j - s.b0) * p.block_size, n = min(p.block_size, s.k1 - t0);
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(1024) void select_rows_kernel(BlockAttnArgs p, SeqT
   extern __shared__ __align__(16) float scores[];
   __shared__ int unsettled[64];
   __shared__ float qs[kMaxHeadDim];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int hk = blockIdx.x % p.kv_heads, wg = blockIdx.x / p.kv_heads, each = p.heads / p.kv_heads;
   const int b = seq_of(t, t.ct, 3, wg);
   const int q0 = table_at(t, t.cu_q, 0, b), q1 = table_at(t, t.cu_q, 0, b + 1);
@@ -553,7 +553,7 @@ __global__ __launch_bounds__(512) void attention_rows_kernel(BlockAttnArgs p, Se
   constexpr int IT = LPK < 16 ? LPK : 16;    // loads per round
   constexpr int KR = IT * KPI;               // keys per round: 64, or 32 with every score in two lanes
   __shared__ float part_o[8][DH], part_m[8], part_l[8];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int row = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
   const int hk = head / (p.heads / p.kv_heads), dim = p.head_dim;
   const Seq s = seq_at(t, seq_of(t, t.cu_q, 0, row));
@@ -853,7 +853,7 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
   constexpr int KS = DH / 32;
   __shared__ __align__(16) uint8_t tile_k[PL * kPlane], tile_v[PL * kPlane];
   __shared__ float tile_max[2][4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lg = lane >> 4;
   // Workgroup i runs on XCD i % 8, and each XCD has its own L2: an XCD takes an
   // eighth of the tiles one after the other, two or three key heads' of 20, and

@@ -355,11 +355,14 @@ struct LinearI4Args {
   int tiles_k = 0;  // ceil(K / 128)
   bool vec_a = false;  // A's rows start at 16-byte addresses
 };
-// How linear_i4 runs: 16 row_tiles rows at a time with the activations split in
-// the kernel, or as a GEMM on activations split into scratch beforehand.
+// How linear_i4 runs: up to 16 rows with the activations split in the kernel, or
+// on activations split into scratch beforehand, in small tiles with the inputs
+// spread over the waves or as a GEMM.
 struct LinearI4Plan {
-  bool gemm = false;
-  int row_tiles = 1;
+  enum Form { kRows, kMid, kGemm } form = kRows;
+  int col_tiles = 1;  // kRows: 16-column tiles per workgroup
+  int waves = 1;      // kRows, kMid
+  int chunk = 1;      // kRows: 128-input tiles whose activations are in LDS at a time
   size_t scratch_bytes = 0;
 };
 LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type);

@@ -84,105 +84,151 @@ __device__ __forceinline__ void load8(const T* row, int k, int K, bool vec, T (&
   }
 }
 
+// Four consecutive outputs of row m from column n on, with their bias.
+template <class T>
+__device__ __forceinline__ void store4(const LinearI4Args& p, int m, int n, f32x4 sum) {
+  if (m >= p.M) return;
+  T* c = static_cast<T*>(p.C) + static_cast<size_t>(m) * p.ldc + n;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < p.N) c[i] = static_cast<T>(sum[i] + (p.bias ? p.bias[n + i] : 0.0f));
+}
+
 // The exponent e for which amax * 2^e lies in [2^14, 2^15) (amax finite;
 // limited to what 2^e and 2^-e can be).
 __device__ __forceinline__ int row_exponent(float amax) {
   return amax > 0.0f ? max(-120, min(120, 15 - __builtin_amdgcn_frexp_expf(amax))) : 0;
 }
 
+// Eight values of a row's 128, the others in the lane's group of 16, as fp16 hi
+// (and lo) operands of the scaled values; *inv receives the scale's inverse. An
+// infinity stays one (its lo part is zero), the others are scaled without it.
+template <int PL>
+__device__ __forceinline__ void split_scaled(const float (&x)[8], uint4 (&out)[PL], float* inv) {
+  auto over_lanes = [](float v) {
+    v = fmaxf(v, lane_dpp<0x128>(v));  // row_ror:8
+    v = fmaxf(v, lane_dpp<0x124>(v));  // row_ror:4
+    v = fmaxf(v, lane_dpp<0x4e>(v));   // quad_perm [2, 3, 0, 1]
+    return fmaxf(v, lane_dpp<0xb1>(v));  // quad_perm [1, 0, 3, 2]
+  };
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2)  // one instruction for two (fmaxf quiets its operands first)
+    asm("v_max3_f32 %0, |%1|, |%2|, %0" : "+v"(amax) : "v"(x[i]), "v"(x[i + 1]));
+  amax = over_lanes(amax);
+  const bool finite = amax < INFINITY;
+  if (__builtin_amdgcn_ballot_w64(!finite)) {
+    float fmax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) fmax = fmaxf(fmax, fabsf(x[i]) < INFINITY ? fabsf(x[i]) : 0.0f);
+    amax = over_lanes(fmax);
+  }
+  const int e = row_exponent(amax);
+  const float mul = __builtin_amdgcn_ldexpf(1.0f, e);
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split_pair(x[2 * i] * mul, x[2 * i + 1] * mul, &h[i], &l[i]);
+  out[0] = make_uint4(h[0], h[1], h[2], h[3]);
+  if constexpr (PL == 2) {
+    if (__builtin_amdgcn_ballot_w64(!finite)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (fabsf(x[i]) == INFINITY) l[i >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
+    }
+    out[PL - 1] = make_uint4(l[0], l[1], l[2], l[3]);
+  }
+  *inv = __builtin_amdgcn_ldexpf(1.0f, -e);
+}
+
 }  // namespace
 
-// One workgroup: 16 MT rows x 16 NT outputs, its NW waves taking the 128-input
-// tiles in turn and adding up through LDS. D = W x^T, so that a lane's outputs
-// are four consecutive ones of the row l % 16 whose activations it also holds:
-// the row's power of two needs no exchange, and a store is 16 bytes.
-template <int DT, int MT, int NT, int GJ>  // GJ: 32-input steps of a group within a tile (1, 2 or 4)
-__global__ __launch_bounds__(512) void linear_i4_rows_kernel(LinearI4Args p) {
+// ------------------------------------------------------------- up to 16 rows
+// One workgroup: all rows x 16 NT outputs, its waves taking the 128-input tiles in
+// turn and adding up through LDS. The workgroup splits the activations into LDS
+// once, every lane eight inputs of its own (as operands loaded and split in each
+// lane, 16 lanes would do one row's work over again: 1 x 10,240 x 2,560 13 us
+// instead of 8), while the first tile's codes and scales are on their way; a
+// tile's are loaded while the tile before is computed. D = W x^T, so that a
+// lane's outputs are four consecutive ones of one row.
+template <int DT, int NT, int GJ>  // GJ: 32-input steps of a group within a tile (1, 2 or 4)
+__global__ __launch_bounds__(1024) void linear_i4_rows_kernel(LinearI4Args p, int chunk) {
   using T = typename Elem<DT>::T;
   constexpr int PL = Elem<DT>::kPlanes;
-  extern __shared__ float red[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  constexpr int kTileBytes = PL * 256;  // a row's 128 inputs
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int lr = lane & 15, kq = lane >> 4;
-  const int cols = (p.N + 16 * NT - 1) / (16 * NT);
-  const int n0 = blockIdx.x % cols * (16 * NT), m0 = blockIdx.x / cols * (16 * MT);
-  const int tiles_n = (p.N + kTileN - 1) / kTileN;
-  const T* rows[MT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int m = m0 + 16 * mt + lr;
-    rows[mt] = m < p.M ? static_cast<const T*>(p.A) + static_cast<size_t>(m) * p.lda : nullptr;
-  }
-  f32x4 total[NT][MT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) total[nt][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  for (int kt = wave; kt < p.tiles_k; kt += waves) {
+  const int tn0 = blockIdx.x * NT, tiles_n = (p.N + kTileN - 1) / kTileN;
+  const int pitch = chunk * kTileBytes + 16;  // rows of 16-byte pieces on distinct banks
+  float* inv = reinterpret_cast<float*>(lds + p.M * pitch);  // [chunk][M]
+  struct Tile {
     u32x4 w[NT];
+    f32x4 s[NT][4 / GJ];
+  };
+  auto load = [&](int kt, Tile& t) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int tn = min(n0 / kTileN + nt, tiles_n - 1);
-      w[nt] = reinterpret_cast<const u32x4*>(p.W)[(static_cast<size_t>(tn) * p.tiles_k + kt) * 64 + lane];
-    }
-    f16x8 a[MT][4][PL];
-    float inv[MT];
+      const int tn = min(tn0 + nt, tiles_n - 1);
+      t.w[nt] = reinterpret_cast<const u32x4*>(p.W)[(static_cast<size_t>(tn) * p.tiles_k + kt) * 64 + lane];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      T x[4][8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) load8<T>(rows[mt], kt * kTileK + 32 * j + 8 * kq, p.K, p.vec_a, x[j]);
-      inv[mt] = 1.0f;
-      if constexpr (DT == kTypeF16) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) __builtin_memcpy(&a[mt][j][0], x[j], 16);
-      } else {
-        float amax = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float v = fabsf(static_cast<float>(x[j][i]));
-            amax = fmaxf(amax, v < INFINITY ? v : 0.0f);
-          }
-        const LanePair s = lane_xor16(amax);
-        amax = fmaxf(s.a, s.b);
-        const LanePair t = lane_xor32(amax);
-        amax = fmaxf(t.a, t.b);
-        const int e = row_exponent(amax);
-        const float mul = __builtin_amdgcn_ldexpf(1.0f, e);
-        inv[mt] = __builtin_amdgcn_ldexpf(1.0f, -e);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float v = static_cast<float>(x[j][i]) * mul;
-            const _Float16 hi = static_cast<_Float16>(v);
-            a[mt][j][0][i] = hi;
-            if constexpr (PL == 2) a[mt][j][PL - 1][i] = static_cast<_Float16>(fabsf(v) < INFINITY ? v - static_cast<float>(hi) : 0.0f);
-          }
+      for (int g = 0; g < 4 / GJ; ++g) {
+        const int group = min((kt * kTileK + g * 32 * GJ) / p.group, p.groups - 1);
+        t.s[nt][g] = *reinterpret_cast<const f32x4*>(p.scales + (static_cast<size_t>(tn) * p.groups + group) * kTileN + 4 * kq);
       }
     }
+  };
+  f32x4 total[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int tn = min(n0 / kTileN + nt, tiles_n - 1);
-      f32x4 acc[MT];
+  for (int nt = 0; nt < NT; ++nt) total[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  Tile next;
+  if (wave < p.tiles_k) load(wave, next);
+  for (int c0 = 0; c0 < p.tiles_k; c0 += chunk) {  // chunk: a multiple of the waves, or all tiles
+    const int n = min(chunk, p.tiles_k - c0);
+    if (c0 > 0) __syncthreads();
+    // 16 lanes to a tile of a row.
+    for (int u = wave * 4 + kq; u < n * p.M; u += waves * 4) {
+      const int tile = u / p.M, m = u - tile * p.M;
+      T x[8];
+      load8<T>(static_cast<const T*>(p.A) + static_cast<size_t>(m) * p.lda, (c0 + tile) * kTileK + 8 * lr, p.K, p.vec_a, x);
+      uint4 out[PL];
+      float unit = 1.0f;
+      if constexpr (DT == kTypeF16) {
+        __builtin_memcpy(&out[0], x, 16);
+      } else {
+        float f[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f16x8 wf = unpack_codes(w[nt][j]);
+        for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(x[i]);
+        split_scaled<PL>(f, out, &unit);
+      }
+      uint8_t* at = lds + m * pitch + tile * kTileBytes + lr * 16;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          acc[mt] = mma(wf, a[mt][j][0], j % GJ == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[mt]);
-          if constexpr (PL == 2) acc[mt] = mma(wf, a[mt][j][PL - 1], acc[mt]);
-        }
-        if ((j + 1) % GJ == 0) {
-          const int g = min((kt * kTileK + 32 * j) / p.group, p.groups - 1);
-          const f32x4 s = *reinterpret_cast<const f32x4*>(p.scales + (static_cast<size_t>(tn) * p.groups + g) * kTileN + 4 * kq);
+      for (int pl = 0; pl < PL; ++pl) *reinterpret_cast<uint4*>(at + pl * 256) = out[pl];
+      if (lr == 0) inv[tile * p.M + m] = unit;
+    }
+    __syncthreads();
+    const int m = min(lr, p.M - 1);  // lanes past the last row take it again; their outputs are not stored
+    for (int tile = wave; tile < n; tile += waves) {
+      const Tile t = next;
+      if (c0 + tile + waves < p.tiles_k) load(c0 + tile + waves, next);
+      const uint8_t* at = lds + m * pitch + tile * kTileBytes + kq * 16;
+      f16x8 a[4][PL];
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              total[nt][mt][i] = __builtin_fmaf(acc[mt][i], s[i] * inv[mt], total[nt][mt][i]);
+        for (int pl = 0; pl < PL; ++pl) a[j][pl] = *reinterpret_cast<const f16x8*>(at + pl * 256 + j * 64);
+      const float unit = inv[tile * p.M + m];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        f32x4 acc;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f16x8 wf = unpack_codes(t.w[nt][j]);
+          acc = mma(wf, a[j][0], j % GJ == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc);
+          if constexpr (PL == 2) acc = mma(wf, a[j][PL - 1], acc);
+          if ((j + 1) % GJ == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) total[nt][i] = __builtin_fmaf(acc[i], t.s[nt][j / GJ][i] * unit, total[nt][i]);
           }
         }
       }
@@ -190,21 +236,15 @@ __global__ __launch_bounds__(512) void linear_i4_rows_kernel(LinearI4Args p) {
   }
 
   // The waves' sums meet in LDS and are added in the waves' order.
-  f32x4* out4 = reinterpret_cast<f32x4*>(red);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) out4[(wave * NT * MT + nt * MT + mt) * 64 + lane] = total[nt][mt];
   __syncthreads();
-  for (int u = wave; u < NT * MT; u += waves) {
-    f32x4 sum = out4[u * 64 + lane];
-    for (int w = 1; w < waves; ++w) sum += out4[(w * NT * MT + u) * 64 + lane];
-    const int m = m0 + 16 * (u % MT) + lr, n = n0 + 16 * (u / MT) + 4 * kq;
-    if (m >= p.M || n >= p.N) continue;
-    T* c = static_cast<T*>(p.C) + static_cast<size_t>(m) * p.ldc + n;
+  f32x4* out4 = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < p.N) c[i] = static_cast<T>(sum[i] + (p.bias ? p.bias[n + i] : 0.0f));
+  for (int nt = 0; nt < NT; ++nt) out4[(wave * NT + nt) * 64 + lane] = total[nt];
+  __syncthreads();
+  for (int u = wave; u < NT; u += waves) {
+    f32x4 sum = out4[u * 64 + lane];
+    for (int w = 1; w < waves; ++w) sum += out4[(w * NT + u) * 64 + lane];
+    store4<T>(p, lr, (tn0 + u) * kTileN + 4 * kq, sum);
   }
 }
 
@@ -257,6 +297,97 @@ __global__ __launch_bounds__(256) void linear_i4_split_kernel(LinearI4Args p, ui
   }
 }
 
+// 16 MT rows x 16 NT outputs per workgroup, for grids that larger tiles would
+// leave empty: the waves take the 128-input tiles in turn, each straight from
+// memory into its operand registers while the one before is computed, and add up
+// through LDS.
+template <int DT, int MT, int NT, int GJ>
+__global__ __launch_bounds__(512) void linear_i4_mid_kernel(LinearI4Args p, const uint16_t* planes, const float* inv,
+                                                            int ldp) {
+  using T = typename Elem<DT>::T;
+  constexpr int PL = Elem<DT>::kPlanes;
+  extern __shared__ float red[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int lr = lane & 15, kq = lane >> 4;
+  const int cols = (p.N + 16 * NT - 1) / (16 * NT), tiles_n = (p.N + kTileN - 1) / kTileN;
+  const int tn0 = blockIdx.x % cols * NT, m0 = blockIdx.x / cols * (16 * MT);
+  const uint16_t* rows[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+    rows[mt] = planes + static_cast<size_t>(min(m0 + 16 * mt + lr, p.M - 1)) * ldp + 8 * kq;
+  const size_t plane = static_cast<size_t>(p.M) * ldp;
+  struct Tile {
+    u32x4 w[NT];
+    f32x4 s[NT][4 / GJ];
+    f16x8 a[MT][4][PL];
+  };
+  auto load = [&](int kt, Tile& t) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int tn = min(tn0 + nt, tiles_n - 1);
+      t.w[nt] = reinterpret_cast<const u32x4*>(p.W)[(static_cast<size_t>(tn) * p.tiles_k + kt) * 64 + lane];
+#pragma unroll
+      for (int g = 0; g < 4 / GJ; ++g) {
+        const int group = min((kt * kTileK + g * 32 * GJ) / p.group, p.groups - 1);
+        t.s[nt][g] = *reinterpret_cast<const f32x4*>(p.scales + (static_cast<size_t>(tn) * p.groups + group) * kTileN + 4 * kq);
+      }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int pl = 0; pl < PL; ++pl)
+          t.a[mt][j][pl] = *reinterpret_cast<const f16x8*>(rows[mt] + pl * plane + kt * kTileK + 32 * j);
+  };
+  f32x4 total[NT][MT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) total[nt][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Tile next;
+  if (wave < p.tiles_k) load(wave, next);
+  for (int kt = wave; kt < p.tiles_k; kt += waves) {
+    const Tile t = next;
+    if (kt + waves < p.tiles_k) load(kt + waves, next);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      f32x4 acc[MT];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f16x8 wf = unpack_codes(t.w[nt][j]);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          acc[mt] = mma(wf, t.a[mt][j][0], j % GJ == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[mt]);
+          if constexpr (PL == 2) acc[mt] = mma(wf, t.a[mt][j][PL - 1], acc[mt]);
+        }
+        if ((j + 1) % GJ == 0) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              total[nt][mt][i] = __builtin_fmaf(acc[mt][i], t.s[nt][j / GJ][i], total[nt][mt][i]);
+        }
+      }
+    }
+  }
+  f32x4* out4 = reinterpret_cast<f32x4*>(red);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) out4[(wave * NT * MT + nt * MT + mt) * 64 + lane] = total[nt][mt];
+  __syncthreads();
+  for (int u = wave; u < NT * MT; u += waves) {
+    f32x4 sum = out4[u * 64 + lane];
+    for (int w = 1; w < waves; ++w) sum += out4[(w * NT * MT + u) * 64 + lane];
+    const int m = m0 + 16 * (u % MT) + lr;
+    const float unit = inv[min(m, p.M - 1)];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] *= unit;
+    store4<T>(p, m, (tn0 + u / MT) * kTileN + 4 * kq, sum);
+  }
+}
+
 // 128 x 128 outputs per workgroup, 64 x 64 per wave on v_mfma_f32_32x32x16_f16:
 // activations through LDS by direct loads, 64 inputs a stage, two stages; codes
 // straight from global memory into the operand registers, the next 128 inputs'
@@ -271,7 +402,7 @@ __global__ __launch_bounds__(256) void linear_i4_gemm_kernel(LinearI4Args p, con
   constexpr int kPlaneBytes = kGemmM * kGemmK * 2;
   typedef float f32x16 __attribute__((ext_vector_type(16)));
   __shared__ __align__(1024) uint8_t stage[2][PL * kPlaneBytes];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, half = lane >> 5;
   int m0, n0;
   tile_origin_of(blockIdx.x, p.M, p.N, kGemmM, kGemmN, &m0, &n0);
@@ -407,57 +538,83 @@ __global__ __launch_bounds__(256) void linear_i4_gemm_kernel(LinearI4Args p, con
 
 namespace {
 
-template <int DT, int MT, int NT>
-hipError_t launch_rows(const LinearI4Args& p, hipStream_t s) {
-  const int waves = std::min(NT * MT >= 16 ? 4 : 8, p.tiles_k);
-  const unsigned grid =
-      static_cast<unsigned>((p.N + 16 * NT - 1) / (16 * NT)) * ((p.M + 16 * MT - 1) / (16 * MT));
-  const size_t lds = static_cast<size_t>(waves) * NT * MT * 1024;
-  const dim3 block(64 * waves);
-  if (p.group == 32)
-    linear_i4_rows_kernel<DT, MT, NT, 1><<<grid, block, lds, s>>>(p);
-  else if (p.group == 64)
-    linear_i4_rows_kernel<DT, MT, NT, 2><<<grid, block, lds, s>>>(p);
-  else
-    linear_i4_rows_kernel<DT, MT, NT, 4><<<grid, block, lds, s>>>(p);
+// The kernel of a group's 32-input steps within 128 inputs.
+#define ESM_I4_BY_GROUP(KERNEL, ...)           \
+  do {                                         \
+    if (p.group == 32)                         \
+      KERNEL(1, __VA_ARGS__);                  \
+    else if (p.group == 64)                    \
+      KERNEL(2, __VA_ARGS__);                  \
+    else                                       \
+      KERNEL(4, __VA_ARGS__);                  \
+  } while (0)
+
+template <int DT, int NT>
+hipError_t launch_rows(const LinearI4Args& p, const LinearI4Plan& plan, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>((p.N + 16 * NT - 1) / (16 * NT)), block = 64 * plan.waves;
+  const size_t row_bytes = static_cast<size_t>(plan.chunk) * (Elem<DT>::kPlanes * 256 + 4) + 16;
+  const size_t lds = std::max(p.M * row_bytes, static_cast<size_t>(plan.waves) * NT * 1024);
+#define KERNEL(GJ, _) linear_i4_rows_kernel<DT, NT, GJ><<<grid, block, lds, s>>>(p, plan.chunk)
+  ESM_I4_BY_GROUP(KERNEL, 0);
+#undef KERNEL
   return hipGetLastError();
 }
 
-template <int DT>
-hipError_t launch_gemm(const LinearI4Args& p, void* scratch, hipStream_t s) {
-  const int ldp = p.tiles_k * kTileK;
-  auto* planes = static_cast<uint16_t*>(scratch);
-  auto* inv = reinterpret_cast<float*>(planes + static_cast<size_t>(Elem<DT>::kPlanes) * p.M * ldp);
-  linear_i4_split_kernel<DT><<<p.M, 256, 0, s>>>(p, planes, inv, ldp);
+template <int DT, int GJ>
+void launch_mid(const LinearI4Args& p, const LinearI4Plan& plan, const uint16_t* planes, const float* inv, int ldp,
+                hipStream_t s) {
+  // Two tiles in flight have to fit the registers.
+  constexpr int MT = 2, NT = Elem<DT>::kPlanes == 2 || GJ == 1 ? 2 : 4;
   const unsigned grid =
-      static_cast<unsigned>((p.M + kGemmM - 1) / kGemmM) * static_cast<unsigned>((p.N + kGemmN - 1) / kGemmN);
-  if (p.group == 32)
-    linear_i4_gemm_kernel<DT, 1><<<grid, 256, 0, s>>>(p, planes, inv, ldp);
-  else if (p.group == 64)
-    linear_i4_gemm_kernel<DT, 2><<<grid, 256, 0, s>>>(p, planes, inv, ldp);
-  else
-    linear_i4_gemm_kernel<DT, 4><<<grid, 256, 0, s>>>(p, planes, inv, ldp);
-  return hipGetLastError();
+      static_cast<unsigned>((p.N + 16 * NT - 1) / (16 * NT)) * ((p.M + 16 * MT - 1) / (16 * MT));
+  const size_t lds = static_cast<size_t>(plan.waves) * NT * MT * 1024;
+  linear_i4_mid_kernel<DT, MT, NT, GJ><<<grid, 64 * plan.waves, lds, s>>>(p, planes, inv, ldp);
 }
 
 template <int DT>
 hipError_t launch_typed(const LinearI4Args& p, const LinearI4Plan& plan, void* scratch, hipStream_t s) {
-  if (plan.gemm) return launch_gemm<DT>(p, scratch, s);
-  if (plan.row_tiles == 1) return launch_rows<DT, 1, 1>(p, s);
-  if (plan.row_tiles == 2) return launch_rows<DT, 2, 2>(p, s);
-  return launch_rows<DT, 4, 4>(p, s);
+  if (plan.form == LinearI4Plan::kRows) return plan.col_tiles == 1 ? launch_rows<DT, 1>(p, plan, s) : launch_rows<DT, 2>(p, plan, s);
+  const int ldp = p.tiles_k * kTileK;
+  auto* planes = static_cast<uint16_t*>(scratch);
+  auto* inv = reinterpret_cast<float*>(planes + static_cast<size_t>(Elem<DT>::kPlanes) * p.M * ldp);
+  linear_i4_split_kernel<DT><<<p.M, 256, 0, s>>>(p, planes, inv, ldp);
+  if (plan.form == LinearI4Plan::kMid) {
+#define KERNEL(GJ, _) launch_mid<DT, GJ>(p, plan, planes, inv, ldp, s)
+    ESM_I4_BY_GROUP(KERNEL, 0);
+#undef KERNEL
+  } else {
+    const unsigned grid =
+        static_cast<unsigned>((p.M + kGemmM - 1) / kGemmM) * static_cast<unsigned>((p.N + kGemmN - 1) / kGemmN);
+#define KERNEL(GJ, _) linear_i4_gemm_kernel<DT, GJ><<<grid, 256, 0, s>>>(p, planes, inv, ldp)
+    ESM_I4_BY_GROUP(KERNEL, 0);
+#undef KERNEL
+  }
+  return hipGetLastError();
 }
 
 }  // namespace
 
 LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type) {
   LinearI4Plan plan;
+  const size_t tiles_n = (static_cast<size_t>(p.N) + kTileN - 1) / kTileN, cus = static_cast<size_t>(device_cus());
   const int ldp = p.tiles_k * kTileK;
-  // A tile's 128 rows are 32-bit offsets apart.
-  plan.gemm = p.M > 256 && ldp < (1 << 23);
-  plan.row_tiles = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
-  if (plan.gemm)
-    plan.scratch_bytes = static_cast<size_t>(p.M) * (static_cast<size_t>(ldp) * (type == kTypeF32 ? 4 : 2) + 4);
+  if (p.M <= 16) {
+    plan.form = LinearI4Plan::kRows;
+    plan.col_tiles = tiles_n >= 2 * cus ? 2 : 1;
+    // As many waves as give each the same number of tiles, at most 10, and as many
+    // of the waves' tiles at a time as keep the activations in 60 KB of LDS.
+    const int rounds = (p.tiles_k + 9) / 10;
+    plan.waves = (p.tiles_k + rounds - 1) / rounds;
+    const int fit = static_cast<int>((size_t{60} << 10) / (p.M * ((type == kTypeF32 ? 512 : 256) + 4) + 16));
+    plan.chunk = fit >= p.tiles_k ? p.tiles_k : fit / plan.waves * plan.waves;
+    if (plan.chunk == 0) plan.chunk = plan.waves = std::max(1, fit);
+    return plan;
+  }
+  // A GEMM tile's 128 rows are 32-bit offsets apart.
+  const size_t gemm_tiles = ((static_cast<size_t>(p.M) + kGemmM - 1) / kGemmM) * ((static_cast<size_t>(p.N) + kGemmN - 1) / kGemmN);
+  plan.form = gemm_tiles >= cus / 2 && ldp < (1 << 23) ? LinearI4Plan::kGemm : LinearI4Plan::kMid;
+  plan.waves = std::min(8, p.tiles_k);
+  plan.scratch_bytes = static_cast<size_t>(p.M) * (static_cast<size_t>(ldp) * (type == kTypeF32 ? 4 : 2) + 4);
   return plan;
 }
 
