@@ -251,8 +251,9 @@ __global__ __launch_bounds__(1024) void linear_i4_rows_kernel(LinearI4Args p, in
 // ------------------------------------------------------------- many rows
 // Activations as the matrix cores take them, written once for every column tile:
 // fp16 planes [planes][M][ldp] (hi, and lo for fp32), zeros past K, a row scaled
-// by the power of two that brings its largest to [2^14, 2^15) (fp16 rows are
-// taken as they are), the power's inverse in inv. One workgroup per row.
+// by the power of two that brings its largest to [2^14, 2^15), the power's inverse
+// in inv; fp16 rows as they are, where their alignment or length keeps the
+// kernels from reading them in place. One workgroup per row.
 template <int DT>
 __global__ __launch_bounds__(256) void linear_i4_split_kernel(LinearI4Args p, uint16_t* planes, float* inv, int ldp) {
   using T = typename Elem<DT>::T;
@@ -279,8 +280,6 @@ __global__ __launch_bounds__(256) void linear_i4_split_kernel(LinearI4Args p, ui
     const int e = row_exponent(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
     mul = __builtin_amdgcn_ldexpf(1.0f, e);
     if (threadIdx.x == 0) inv[m] = __builtin_amdgcn_ldexpf(1.0f, -e);
-  } else {
-    if (threadIdx.x == 0) inv[m] = 1.0f;
   }
   for (int k = threadIdx.x * 8; k < ldp; k += 2048) {
     T x[8];
@@ -381,19 +380,24 @@ __global__ __launch_bounds__(512) void linear_i4_mid_kernel(LinearI4Args p, cons
     f32x4 sum = out4[u * 64 + lane];
     for (int w = 1; w < waves; ++w) sum += out4[(w * NT * MT + u) * 64 + lane];
     const int m = m0 + 16 * (u % MT) + lr;
-    const float unit = inv[min(m, p.M - 1)];
+    const float unit = inv ? inv[min(m, p.M - 1)] : 1.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum[i] *= unit;
     store4<T>(p, m, (tn0 + u / MT) * kTileN + 4 * kq, sum);
   }
 }
 
-// 128 x 128 outputs per workgroup, 64 x 64 per wave on v_mfma_f32_32x32x16_f16:
+// 64 x 256 outputs per workgroup, 64 x 64 per wave on v_mfma_f32_32x32x16_f16:
 // activations through LDS by direct loads, 64 inputs a stage, two stages; codes
 // straight from global memory into the operand registers, the next 128 inputs'
 // on their way. D has outputs across lanes: a group's scale is one register per
-// 32 columns.
-constexpr int kGemmM = 128, kGemmN = 128, kGemmK = 64;
+// 32 columns. The tile is wide because a row of split fp32 activations costs four
+// bytes an input and a column of codes half a byte, and low so that two
+// workgroups share a CU, one storing while the other multiplies: 4,099 x 5,120 x
+// 1,280 took 139 us in 128 x 128 tiles, 132 in 128 x 256 and 129 in these. At
+// 107 GFLOP of fp16 products (two per fp32 one) that is 830 TFLOP/s, 1,150 without
+// the stores (84 MB, 12 us on their own) and the last, partly empty round.
+constexpr int kGemmM = 64, kGemmN = 256, kGemmK = 64;
 template <int DT, int GJ>  // GJ: 32-input steps of a group within 128 inputs
 __global__ __launch_bounds__(256) void linear_i4_gemm_kernel(LinearI4Args p, const uint16_t* planes, const float* inv,
                                                              int ldp) {
@@ -406,26 +410,25 @@ __global__ __launch_bounds__(256) void linear_i4_gemm_kernel(LinearI4Args p, con
   const int ln = lane & 31, half = lane >> 5;
   int m0, n0;
   tile_origin_of(blockIdx.x, p.M, p.N, kGemmM, kGemmN, &m0, &n0);
-  const int wm = wave >> 1, wn = wave & 1;
 
   // Direct loads: one instruction brings 8 rows of 64 inputs (1 KB); wave w loads
-  // rows 32 w .. + 32. The 16-byte piece c of row r lies at c ^ (r % 8), so that
-  // 32 rows' pieces fall on distinct banks.
+  // rows 16 w .. + 16. The 16-byte piece c of row r lies at c ^ (r / 2 % 8), so that
+  // 16 rows' pieces fall on distinct banks.
   const uint32_t lds0 = lds_byte_addr(&stage[0][0]);
-  uint32_t off[4];
+  uint32_t off[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = wave * 32 + i * 8 + (lane >> 3), c = (lane & 7) ^ (lane >> 3);
+  for (int i = 0; i < 2; ++i) {
+    const int r = wave * 16 + i * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
     off[i] = static_cast<uint32_t>(min(r, p.M - 1 - m0)) * static_cast<uint32_t>(ldp * 2) + c * 16;
   }
-  const size_t plane_elems = static_cast<size_t>(p.M) * ldp;
+  const size_t plane_elems = PL == 2 ? static_cast<size_t>(p.M) * ldp : 0;
   auto load_stage = [&](int k0, int buf) {
 #pragma unroll
     for (int pl = 0; pl < PL; ++pl) {
       const uint16_t* base = planes + pl * plane_elems + static_cast<size_t>(m0) * ldp + k0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        lds_dma16(base, off[i], lds0 + buf * (PL * kPlaneBytes) + pl * kPlaneBytes + (wave * 32 + i * 8) * 128);
+      for (int i = 0; i < 2; ++i)
+        lds_dma16(base, off[i], lds0 + buf * (PL * kPlaneBytes) + pl * kPlaneBytes + (wave * 16 + i * 8) * 128);
     }
   };
 
@@ -436,7 +439,7 @@ __global__ __launch_bounds__(256) void linear_i4_gemm_kernel(LinearI4Args p, con
   const float* sp[2];
 #pragma unroll
   for (int nt = 0; nt < 2; ++nt) {
-    const int tn = min((n0 + wn * 64 + nt * 32) / kTileN + (ln >> 4), tiles_n - 1);
+    const int tn = min((n0 + wave * 64 + nt * 32) / kTileN + (ln >> 4), tiles_n - 1);
     wp[nt] = reinterpret_cast<const u32x4*>(p.W) + static_cast<size_t>(tn) * p.tiles_k * 64 + (ln & 15) + 16 * half;
     sp[nt] = p.scales + static_cast<size_t>(tn) * p.groups * kTileN + (ln & 15);
   }
@@ -481,31 +484,34 @@ __global__ __launch_bounds__(256) void linear_i4_gemm_kernel(LinearI4Args p, con
         load_stage((kt + 1) * kTileK, 0);
         load_codes(kt + 1, wnext, snext);
       }
-      const uint8_t* at = stage[h];
-#pragma unroll
-      for (int st = 0; st < 4; ++st) {
+      // Each 16 inputs' operands are read and unpacked while the 16 before are on
+      // the matrix cores.
+      f16x8 a[2][2][PL], wf[2][2];
+      auto operands = [&](int st) {
         const int step = h * 4 + st;  // of the 128 inputs' eight
-        f16x8 wf[2];
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) wf[nt] = unpack_codes(w[nt][step & 1][step >> 1]);
-        const bool first = step % (2 * GJ) == 0;
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
-          const int r = wm * 64 + mt * 32 + ln;
-          const uint8_t* a = at + r * 128 + (((2 * st + half) ^ (r & 7)) << 4);
-          const f16x8 ah = *reinterpret_cast<const f16x8*>(a);
-          f16x8 al;
-          if constexpr (PL == 2) al = *reinterpret_cast<const f16x8*>(a + kPlaneBytes);
+          const int r = mt * 32 + ln;
+          const uint8_t* at = stage[h] + r * 128 + (((2 * st + half) ^ ((r >> 1) & 7)) << 4);
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            if (first) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) acc[mt][nt][i] = 0.0f;
-            }
-            acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, wf[nt], acc[mt][nt], 0, 0, 0);
-            if constexpr (PL == 2) acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, wf[nt], acc[mt][nt], 0, 0, 0);
-          }
+          for (int pl = 0; pl < PL; ++pl) a[st & 1][mt][pl] = *reinterpret_cast<const f16x8*>(at + pl * kPlaneBytes);
         }
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) wf[st & 1][nt] = unpack_codes(w[nt][step & 1][step >> 1]);
+      };
+      operands(0);
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        const int step = h * 4 + st;
+        if (st < 3) operands(st + 1);
+#pragma unroll
+        for (int pl = 0; pl < PL; ++pl)
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+              acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                  a[st & 1][mt][pl], wf[st & 1][nt], step % (2 * GJ) == 0 && pl == 0 ? f32x16{} : acc[mt][nt], 0, 0, 0);
         if (step % (2 * GJ) == 2 * GJ - 1) {
           const int g = step / (2 * GJ);
 #pragma unroll
@@ -516,24 +522,36 @@ __global__ __launch_bounds__(256) void linear_i4_gemm_kernel(LinearI4Args p, con
               for (int i = 0; i < 16; ++i)
                 total[mt][nt][i] = __builtin_fmaf(acc[mt][nt][i], s[nt][g], total[mt][nt][i]);
         }
+#pragma unroll
+        for (int i = 0; i < 4 * PL; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // an MFMA
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // an LDS read
+          __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // vector instructions
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
 
+  // A row's power of two once per row, and no conditions in whole tiles.
+  const bool whole = m0 + kGemmM <= p.M && n0 + kGemmN <= p.N;
+  const int n = n0 + wave * 64 + ln;
+  float bias[2];
 #pragma unroll
-  for (int nt = 0; nt < 2; ++nt) {
-    const int n = n0 + wn * 64 + nt * 32 + ln;
-    const float bias = p.bias && n < p.N ? p.bias[n] : 0.0f;
+  for (int nt = 0; nt < 2; ++nt) bias[nt] = p.bias && n + nt * 32 < p.N ? p.bias[n + nt * 32] : 0.0f;
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+  for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int m = m0 + wm * 64 + mt * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-        if (m < p.M && n < p.N)
-          static_cast<T*>(p.C)[static_cast<size_t>(m) * p.ldc + n] =
-              static_cast<T>(__builtin_fmaf(total[mt][nt][i], inv[m], bias));
+    for (int i = 0; i < 16; ++i) {
+      const int m = m0 + mt * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
+      const float unit = inv ? inv[min(m, p.M - 1)] : 1.0f;
+      T* c = static_cast<T*>(p.C) + static_cast<size_t>(m) * p.ldc + n;
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const T y = static_cast<T>(__builtin_fmaf(total[mt][nt][i], unit, bias[nt]));
+        if (whole || (m < p.M && n + nt * 32 < p.N)) c[nt * 32] = y;
       }
-  }
+    }
 }
 
 namespace {
@@ -574,10 +592,17 @@ void launch_mid(const LinearI4Args& p, const LinearI4Plan& plan, const uint16_t*
 template <int DT>
 hipError_t launch_typed(const LinearI4Args& p, const LinearI4Plan& plan, void* scratch, hipStream_t s) {
   if (plan.form == LinearI4Plan::kRows) return plan.col_tiles == 1 ? launch_rows<DT, 1>(p, plan, s) : launch_rows<DT, 2>(p, plan, s);
-  const int ldp = p.tiles_k * kTileK;
-  auto* planes = static_cast<uint16_t*>(scratch);
-  auto* inv = reinterpret_cast<float*>(planes + static_cast<size_t>(Elem<DT>::kPlanes) * p.M * ldp);
-  linear_i4_split_kernel<DT><<<p.M, 256, 0, s>>>(p, planes, inv, ldp);
+  int ldp = p.lda;
+  const uint16_t* planes = static_cast<const uint16_t*>(p.A);
+  const float* inv = nullptr;
+  if (plan.scratch_bytes) {
+    ldp = p.tiles_k * kTileK;
+    auto* to = static_cast<uint16_t*>(scratch);
+    auto* units = reinterpret_cast<float*>(to + static_cast<size_t>(Elem<DT>::kPlanes) * p.M * ldp);
+    linear_i4_split_kernel<DT><<<p.M, 256, 0, s>>>(p, to, units, ldp);
+    planes = to;
+    inv = DT == kTypeF16 ? nullptr : units;
+  }
   if (plan.form == LinearI4Plan::kMid) {
 #define KERNEL(GJ, _) launch_mid<DT, GJ>(p, plan, planes, inv, ldp, s)
     ESM_I4_BY_GROUP(KERNEL, 0);
@@ -597,7 +622,6 @@ hipError_t launch_typed(const LinearI4Args& p, const LinearI4Plan& plan, void* s
 LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type) {
   LinearI4Plan plan;
   const size_t tiles_n = (static_cast<size_t>(p.N) + kTileN - 1) / kTileN, cus = static_cast<size_t>(device_cus());
-  const int ldp = p.tiles_k * kTileK;
   if (p.M <= 16) {
     plan.form = LinearI4Plan::kRows;
     plan.col_tiles = tiles_n >= 2 * cus ? 2 : 1;
@@ -610,11 +634,16 @@ LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type) {
     if (plan.chunk == 0) plan.chunk = plan.waves = std::max(1, fit);
     return plan;
   }
-  // A GEMM tile's 128 rows are 32-bit offsets apart.
+  // Rows that the kernels can read in place need no scratch.
+  const bool in_place = type == kTypeF16 && p.vec_a && p.K % kTileK == 0;
+  const int ldp = in_place ? p.lda : p.tiles_k * kTileK;
+  // A GEMM tile's 64 rows are 32-bit offsets apart.
   const size_t gemm_tiles = ((static_cast<size_t>(p.M) + kGemmM - 1) / kGemmM) * ((static_cast<size_t>(p.N) + kGemmN - 1) / kGemmN);
-  plan.form = gemm_tiles >= cus / 2 && ldp < (1 << 23) ? LinearI4Plan::kGemm : LinearI4Plan::kMid;
+  plan.form = gemm_tiles >= cus && ldp < (1 << 23) ? LinearI4Plan::kGemm : LinearI4Plan::kMid;
   plan.waves = std::min(8, p.tiles_k);
-  plan.scratch_bytes = static_cast<size_t>(p.M) * (static_cast<size_t>(ldp) * (type == kTypeF32 ? 4 : 2) + 4);
+  if (!in_place)
+    plan.scratch_bytes =
+        static_cast<size_t>(p.M) * (static_cast<size_t>(p.tiles_k) * kTileK * (type == kTypeF32 ? 4 : 2) + 4);
   return plan;
 }
 
