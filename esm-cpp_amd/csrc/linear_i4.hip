@@ -17,6 +17,7 @@
 // into the fp16 pair 1024 + u (or 1024 + 16 u), and one packed add (fma) into
 // the codes: nine instructions for eight weights.
 #include <algorithm>
+#include <cmath>
 
 #include "common.hpp"
 #include "kernels.hpp"
@@ -621,7 +622,7 @@ hipError_t launch_typed(const LinearI4Args& p, const LinearI4Plan& plan, void* s
 
 LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type) {
   LinearI4Plan plan;
-  const size_t tiles_n = (static_cast<size_t>(p.N) + kTileN - 1) / kTileN, cus = static_cast<size_t>(device_cus());
+  const size_t tiles_n = (static_cast<size_t>(p.N) + kTileN - 1) / kTileN, cus = std::max(1, device_cus());
   if (p.M <= 16) {
     plan.form = LinearI4Plan::kRows;
     plan.col_tiles = tiles_n >= 2 * cus ? 2 : 1;
@@ -637,9 +638,24 @@ LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type) {
   // Rows that the kernels can read in place need no scratch.
   const bool in_place = type == kTypeF16 && p.vec_a && p.K % kTileK == 0;
   const int ldp = in_place ? p.lda : p.tiles_k * kTileK;
-  // A GEMM tile's 64 rows are 32-bit offsets apart.
-  const size_t gemm_tiles = ((static_cast<size_t>(p.M) + kGemmM - 1) / kGemmM) * ((static_cast<size_t>(p.N) + kGemmN - 1) / kGemmN);
-  plan.form = gemm_tiles >= cus && ldp < (1 << 23) ? LinearI4Plan::kGemm : LinearI4Plan::kMid;
+  // Both kernels' time on an idle device, in us, as measured over 17 to 2,048 rows
+  // of 1,280 x 1,280, 5,120 x 1,280, 1,280 x 5,120 and 10,240 x 2,560: small tiles
+  // take 3.0 (fp32: 3.9) for each 128-input tile of a wave in each round of one
+  // workgroup per CU; a GEMM workgroup 10 and 0.6 (0.97) per 64 inputs while it has
+  // a CU to itself, 1.4 times that where two share one, and rounds of those. So 256
+  // fp32 rows of 5,120 x 1,280 are a GEMM (32 us, small tiles 41) and 512 of
+  // 1,280 x 5,120 small tiles (72, GEMM 90).
+  const bool two = type == kTypeF32;
+  const int mid_cols = 16 * (two || p.group == 32 ? 2 : 4);
+  const double mid_wgs = static_cast<double>((p.M + 31) / 32) * ((static_cast<size_t>(p.N) + mid_cols - 1) / mid_cols);
+  const double gemm_wgs = static_cast<double>((static_cast<size_t>(p.M) + kGemmM - 1) / kGemmM) *
+                          static_cast<double>((static_cast<size_t>(p.N) + kGemmN - 1) / kGemmN);
+  const double mid_us = (two ? 3.9 : 3.0) * ((p.tiles_k + 7) / 8) * std::ceil(mid_wgs / cus);
+  const double gemm_us = (10.0 + (two ? 0.97 : 0.6) * 2 * p.tiles_k) *
+                         (gemm_wgs <= cus ? 1.0 : 1.4 * std::max(1.0, gemm_wgs / (2.0 * cus)));
+  // A GEMM tile's 64 rows are 32-bit offsets apart, and its grid is one number.
+  const bool gemm_ok = ldp < (1 << 23) && gemm_wgs < 2e9;
+  plan.form = gemm_ok && gemm_us < mid_us ? LinearI4Plan::kGemm : LinearI4Plan::kMid;
   plan.waves = std::min(8, p.tiles_k);
   if (!in_place)
     plan.scratch_bytes =

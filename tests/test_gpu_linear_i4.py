@@ -98,6 +98,39 @@ def test_against_the_formula(dev, kind, M, N, K, group):
     check(dev, kind, M, N, K, group, seed=M * 7 + N + K)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("M,N,K,group", [(700, 5130, 200, 32), (700, 5130, 200, 64), (700, 5130, 256, 128),
+                                         (1030, 2570, 1400, 256)])
+def test_many_rows_and_columns(dev, kind, M, N, K, group):
+    """Sizes at which the products run as a GEMM, with tiles that M, N and K end inside."""
+    check(dev, kind, M, N, K, group, seed=M + N + K + group)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("offset,pad", [(0, 8), (1, 3)])
+def test_strides_of_many_rows_and_columns(dev, kind, offset, pad):
+    M, N, K, group = 650, 5130, 256, 64
+    r = rng(pad)
+    size = 4 if kind == "fp32" else 2
+    packed = r.integers(0, 256, size=(N, K // 2)).astype(np.uint8)
+    scales = r.standard_normal((N, K // group)).astype(np.float32)
+    lda, ldc = K + pad, N + pad
+    x = to_bits(r.standard_normal((M * lda + offset,)).astype(np.float32), kind)
+    x[offset + 3 * lda + 7] = to_bits(np.array([np.inf], np.float32), kind)[0]
+    X, W = dev.array(x), dev.weight_i4(packed, scales, K, group)
+    C = dev.array(empty_as(kind, (M * ldc,), 99))
+    dev.linear_i4(At(X, offset * size), W, None, C, M, N, K, TYPES[kind], lda=lda, ldc=ldc)
+    rows = C.numpy().reshape(M, ldc)
+    xr = to_f64(x[offset:], kind).reshape(M, lda)[:, :K]
+    w = decode(packed, scales, K, group)
+    sane = np.arange(M) != 3
+    want = xr[sane] @ w.T
+    assert np.all(np.abs(to_f64(rows[sane, :N], kind) - want) <= tolerance(xr[sane], w, want, kind))
+    assert not np.any(np.isfinite(to_f64(rows[3, :N], kind)))
+    assert np.all(rows[:, N:] == empty_as(kind, (1,), 99)[0])
+    W.free()
+
+
 @pytest.mark.parametrize("M", [1, 40, 300])
 def test_without_bias(dev, M):
     check(dev, "fp32", M, 70, 200, 64, seed=M, bias=False)
