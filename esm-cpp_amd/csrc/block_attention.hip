@@ -51,9 +51,9 @@ struct GroupedWork {
   int* used = nullptr;         // [groups] tiles of a group (behind counts)
   int* first = nullptr;        // [cells] first entry in list
   int4* tiles = nullptr;       // [groups, group_tiles] (cell, first entry, entries, -), each key head's together
-  int* place = nullptr;        // [entries] place in its cell, -1: does not count
+  int* place = nullptr;        // [entries] place in its cell, then in list; -1: does not count
   int* list = nullptr;         // [entries] by cell
-  float2* part_ml = nullptr;   // [entries of the heads in hand] maximum (base 2) and sum
+  float2* part_ml = nullptr;   // [places of the heads in hand] maximum (base 2) and sum
   float* part_o = nullptr;     // [.., padded head_dim]; one entry more takes what belongs to none
 };
 
@@ -672,9 +672,10 @@ __global__ __launch_bounds__(512) void attention_rows_kernel(BlockAttnArgs p, Se
 // Many rows: the lists are turned round. Every cell (key head, block) gets the
 // entries that list it, and a workgroup multiplies 128 of them with the cell's
 // keys and values on the matrix cores, however few neighbours share a block;
-// each entry's part (maximum, sum, weighted values) is written down by entry,
-// and a last pass joins the entries of a row in the order of its list. So no
-// result depends on the order in which a cell's entries were collected.
+// each entry's part (maximum, sum, weighted values) is written down, a
+// workgroup's together, and a last pass gathers the parts of a row in the order
+// of its list. So no result depends on the order in which a cell's entries were
+// collected.
 //
 // An entry is (token - token0, head, list index) as one number; cells are
 // numbered key head first.
@@ -829,7 +830,10 @@ __global__ __launch_bounds__(kCountThreads) void scatter_entries_kernel(BlockAtt
   }
 #pragma unroll
   for (int u = 0; u < kCountPer; ++u)
-    if (place[u] >= 0) g.list[first[u] + place[u]] = at[u];
+    if (place[u] >= 0) {
+      g.list[first[u] + place[u]] = at[u];
+      g.place[at[u]] = first[u] + place[u];
+    }
 }
 
 // One workgroup per tile of up to 512 entries of a cell, 32 at a time to a wave.
@@ -865,8 +869,7 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
   const int hk = tile.x / p.num_blocks, block = tile.x - hk * p.num_blocks, dim = p.head_dim;
   const Seq s = seq_at(t, seq_of(t, t.cb, 2, block));
   const int key0 = s.k0 + (block - s.b0) * p.block_size, keys = min(p.block_size, s.k1 - key0);
-  const int each = p.heads / p.kv_heads, chunk_heads = (hk1 - hk0) * each;
-  const int no_part = g.tokens * chunk_heads * p.top;
+  const int part0 = hk0 * g.head_entries, no_part = (hk1 - hk0) * g.head_entries;
 
   // Loads the 64 keys from key0 + c on, and their values, into LDS.
   int ke = 0, ve = 0;
@@ -915,8 +918,8 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
     __syncthreads();
   };
 
-  // This lane's two queries of the 128 entries from i0 on, and where their parts go.
-  int entry[2], next_entry[2], part[2];
+  // This lane's two queries of the 128 entries from i0 on.
+  int entry[2], next_entry[2];
   float qx[2][KS][8];
   auto list_at = [&](int i0, int (&to)[2]) {
 #pragma unroll
@@ -933,7 +936,6 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int row = g.by_top(max(of[r], 0)), tok = g.by_heads(row), head = row - tok * p.heads;
-      part[r] = of[r] < 0 ? no_part : (tok * chunk_heads + head - hk0 * each) * p.top + (of[r] - row * p.top);
       const T* q = static_cast<const T*>(p.q) + static_cast<size_t>(g.token0 + tok) * p.ldq + head * dim;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -967,7 +969,7 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
         for (int pl = 0; pl < PL; ++pl) qf[r][ks][pl] = __builtin_bit_cast(f16x8, w[pl]);
       }
     }
-    const int now[2] = {part[0], part[1]};
+    const int now[2] = {entry[0], entry[1]};
     entry[0] = next_entry[0];
     entry[1] = next_entry[1];
     load_q(entry);
@@ -1083,7 +1085,8 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const float sum = group_sum(l[r]);
-      const size_t at = now[r];
+      const int i = i0 + wave * 32 + r * 16 + lr;
+      const size_t at = now[r] < 0 ? no_part : tile.y + i - part0;
       g.part_ml[at] = make_float2(m[r], sum);  // the same from all four lanes
 #pragma unroll
       for (int db = 0; db < DH / 16; ++db)
@@ -1106,15 +1109,16 @@ __global__ __launch_bounds__(256) void join_entries_kernel(BlockAttnArgs p, Grou
   const size_t tok = row / chunk_heads;
   const int head = static_cast<int>(row - tok * chunk_heads) + hk0 * each;
   const int* place = g.place + (tok * p.heads + head) * p.top;
-  const float2* ml = g.part_ml + row * p.top;
+  const int part0 = hk0 * g.head_entries;
   constexpr int kStride = GL * 4 < 32 ? 32 : GL * 4;  // the parts' padded head_dim
-  const float* o = g.part_o + row * p.top * kStride + dl;
+  const float* o = g.part_o + dl;
   float m = -INFINITY, sum = 0.0f;
   f32x4 x = {0.f, 0.f, 0.f, 0.f};
   for (int e0 = 0; e0 < p.top; e0 += GL) {
     const int n = min(GL, p.top - e0);
-    const bool counts = gl < n && place[e0 + gl] >= 0;
-    const float2 v = counts ? ml[e0 + gl] : make_float2(-INFINITY, 0.0f);
+    const int at = gl < n ? place[e0 + gl] - part0 : -1;
+    const bool counts = at >= 0;
+    const float2 v = counts ? g.part_ml[at] : make_float2(-INFINITY, 0.0f);
     float mx = v.x;
 #pragma unroll
     for (int b = 1; b < GL; b *= 2) mx = fmaxf(mx, __shfl_xor(mx, b));
@@ -1126,7 +1130,6 @@ __global__ __launch_bounds__(256) void join_entries_kernel(BlockAttnArgs p, Grou
     sum = __builtin_fmaf(sum, alpha, part);
     m = mn;
     x *= alpha;
-    const float* at = o + static_cast<size_t>(e0) * kStride;
     for (int e = 0; e < n; e += 8) {
       f32x4 y[8];
       float ws[8];
@@ -1134,7 +1137,8 @@ __global__ __launch_bounds__(256) void join_entries_kernel(BlockAttnArgs p, Grou
       for (int k = 0; k < 8; ++k) {
         ws[k] = __shfl(w, min(e + k, n - 1), GL);
         if (e + k >= n) ws[k] = -1.0f;
-        y[k] = *reinterpret_cast<const f32x4*>(at + static_cast<size_t>(min(e + k, n - 1)) * kStride);
+        const int from = __shfl(at, min(e + k, n - 1), GL);
+        y[k] = *reinterpret_cast<const f32x4*>(o + static_cast<size_t>(max(from, 0)) * kStride);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k)
@@ -1232,7 +1236,7 @@ GroupedWork grouped_layout(const BlockAttnArgs& p, const BlockAttnPlan& plan, ch
   const size_t entries = static_cast<size_t>(plan.tokens) * p.heads * p.top, head_entries = entries / p.kv_heads;
   const size_t head_tiles = head_entries / kTileEntries + std::min<size_t>(p.num_blocks, head_entries);
   const int groups = (p.kv_heads + plan.kv_heads - 1) / plan.kv_heads;
-  const size_t parts = static_cast<size_t>(plan.tokens) * plan.kv_heads * (p.heads / p.kv_heads) * p.top;
+  const size_t parts = head_entries * plan.kv_heads;
   GroupedWork g;
   size_t at = 0;
   auto take = [&](size_t n) {
