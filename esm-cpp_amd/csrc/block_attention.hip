@@ -10,6 +10,7 @@
 //                   then -1
 //   out[t, h]     = softmax over the listed blocks' keys of q . k, times v
 #include <algorithm>
+#include <cmath>
 
 #include "common.hpp"
 #include "kernels.hpp"
@@ -1262,8 +1263,8 @@ GroupedWork grouped_layout(const BlockAttnArgs& p, const BlockAttnPlan& plan, ch
 }
 
 template <int DT, int DH>
-hipError_t launch_attention_rows(const BlockAttnArgs& p, const SeqTable& t, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(p.rows) * p.heads, block = 64 * (p.top < 8 ? p.top : 8);
+hipError_t launch_attention_rows(const BlockAttnArgs& p, const SeqTable& t, const BlockAttnPlan& plan, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>(p.rows) * p.heads, block = 64 * plan.waves;
   if (p.vec_kv)
     attention_rows_kernel<DT, DH, true><<<grid, block, 0, s>>>(p, t);
   else
@@ -1324,9 +1325,9 @@ template <int DT>
 hipError_t launch_attention_typed(const BlockAttnArgs& p, const SeqTable& t, const BlockAttnPlan& plan, void* scratch,
                                   hipStream_t s) {
   if (!plan.grouped)
-    return p.head_dim <= 32   ? launch_attention_rows<DT, 32>(p, t, s)
-           : p.head_dim <= 64 ? launch_attention_rows<DT, 64>(p, t, s)
-                              : launch_attention_rows<DT, 128>(p, t, s);
+    return p.head_dim <= 32   ? launch_attention_rows<DT, 32>(p, t, plan, s)
+           : p.head_dim <= 64 ? launch_attention_rows<DT, 64>(p, t, plan, s)
+                              : launch_attention_rows<DT, 128>(p, t, plan, s);
   return p.head_dim <= 32   ? launch_attention_cells<DT, 32>(p, t, plan, scratch, s)
          : p.head_dim <= 64 ? launch_attention_cells<DT, 64>(p, t, plan, scratch, s)
                             : launch_attention_cells<DT, 128>(p, t, plan, scratch, s);
@@ -1334,11 +1335,33 @@ hipError_t launch_attention_typed(const BlockAttnArgs& p, const SeqTable& t, con
 
 }  // namespace
 
-BlockAttnPlan attention_blocks_plan(const BlockAttnArgs& p) {
+BlockAttnPlan attention_blocks_plan(const BlockAttnArgs& p, const int* cu_q, const int* cu_k, int batch, int type) {
   BlockAttnPlan plan;
   const size_t cells = static_cast<size_t>(p.num_blocks) * p.kv_heads;
   const size_t row_entries = static_cast<size_t>(p.heads) * p.top;  // of a token
-  plan.grouped = cells > 0 && cells <= 0x3fffffff && row_entries * p.rows >= 4 * cells;
+  // The entries that can count, and their keys.
+  double entries = 0.0, keys = 0.0;
+  int most = 0;
+  for (int b = 0; b < batch; ++b) {
+    const int n = cu_k[b + 1] - cu_k[b], blocks = n > 0 ? (n - 1) / p.block_size + 1 : 0;
+    const double rows = static_cast<double>(cu_q[b + 1] - cu_q[b]) * p.heads;
+    entries += rows * std::min(p.top, blocks);
+    keys += rows * std::min<double>(static_cast<double>(p.top) * p.block_size, n);
+    most = std::max(most, std::min(p.top, blocks));
+  }
+  plan.waves = std::max(1, std::min(8, most));
+  if (cells == 0 || cells > 0x3fffffff || entries == 0.0) return plan;
+  // Both forms' time in us, as measured over 4 to 768 queries of 8 to 40 heads: row
+  // by row 5 and every entry's keys and values at 7.5 TB/s (from L2); block by block
+  // 24 (six launches), 7.5e-3 for every 32 KB that a workgroup stages and 0.25e-3
+  // for every 32 KB of keys and values that an entry meets in LDS. 20 heads of 64,
+  // fp32, 64 queries over their one block each: 9 and 25; 256 over 4: 80 and 33; 16
+  // over 16 of 250: 45 and 48; 100 over 16 of 250: 181 and 66.
+  const double entry_bytes = keys / entries * p.head_dim * 2 * (type == kTypeF32 ? 4 : 2), unit = entry_bytes / 32768.0;
+  const double hit = cells * (1.0 - std::exp(-entries / cells));
+  const double rows_us = 5.0 + entries * entry_bytes / 7.5e6;
+  const double cells_us = 24.0 + (hit + entries / kTileEntries) * 7.5e-3 * unit + entries * 0.25e-3 * unit;
+  plan.grouped = cells_us < rows_us;
   if (!plan.grouped) return plan;
   // Entry numbers are 32-bit, and lists of 2^26 entries take half a gigabyte.
   plan.tokens = static_cast<int>(std::min<size_t>(p.rows, std::max<size_t>(1, (size_t{1} << 26) / row_entries)));

@@ -1220,7 +1220,7 @@ extern "C" int esm_gfx950_attention_blocks(esm_gfx950_ctx* ctx, const void* q, i
     p.out = out;
     p.vec_q = aligned(q, 16) && static_cast<size_t>(ldq) * size % 16 == 0;
     p.vec_kv = aligned(k, 16) && aligned(v, 16) && static_cast<size_t>(ldkv) * size % 16 == 0;
-    const BlockAttnPlan plan = attention_blocks_plan(p);
+    const BlockAttnPlan plan = attention_blocks_plan(p, cu_q, cu_k, batch_size, dtype);
     SeqTable t;
     void* scratch = nullptr;
     ESM_TRY(stage_sequences(ctx, cu_q, cu_k, batch_size, p, nullptr, plan.scratch_bytes, &t, &scratch));

@@ -420,10 +420,11 @@ hipError_t launch_select_blocks(const BlockAttnArgs& p, const SeqTable& t, const
 // `tokens` tokens and `kv_heads` key heads at a time.
 struct BlockAttnPlan {
   bool grouped = false;
+  int waves = 1;  // row by row
   int tokens = 0, kv_heads = 0;
   size_t scratch_bytes = 0;
 };
-BlockAttnPlan attention_blocks_plan(const BlockAttnArgs& p);
+BlockAttnPlan attention_blocks_plan(const BlockAttnArgs& p, const int* cu_q, const int* cu_k, int batch, int type);
 hipError_t launch_attention_blocks(const BlockAttnArgs& p, const SeqTable& t, const BlockAttnPlan& plan, void* scratch,
                                    int type, hipStream_t s);
 

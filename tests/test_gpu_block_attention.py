@@ -111,6 +111,38 @@ SHAPES = [  # queries, keys, heads, key heads, dim, block, top
     ([150], [900], 2, 2, 64, 256, 2), ([90], [2100], 1, 1, 96, 1024, 2)]
 
 
+LARGE = [  # as SHAPES; enough work that blocks are taken in turn
+    ([600], [600], 20, 20, 64, 64, 4), ([260, 0, 300], [260, 5, 333], 16, 4, 128, 32, 9),
+    ([700], [700], 20, 20, 24, 48, 7), ([400], [1500], 10, 5, 64, 256, 3), ([350, 1], [2100, 1], 8, 8, 96, 1024, 2),
+    ([800], [801], 20, 20, 32, 16, 20)]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("shape", LARGE, ids=[str(i) for i in range(len(LARGE))])
+def test_many_rows(dev, kind, shape):
+    """A sample of the rows against the formula, lists of every sort."""
+    q_lens, k_lens, H, Hkv, dim, block, top = shape
+    b = Batch(dev, kind, q_lens, k_lens, H, Hkv, dim, block, seed=sum(k_lens))
+    r = rng(dim)
+    most = int(np.max(np.diff(b.cb)))
+    blocks = r.integers(-1, most + 1, size=(b.rows, H, top)).astype(np.int32)
+    blocks[::3] = np.sort(blocks[::3], axis=2)
+    blocks[7] = -1
+    blocks[:, 1, 0] = 0
+    got = to_f64(b.attend(blocks, top), kind).reshape(b.rows, H, dim)
+    assert np.all(np.isfinite(got)) and np.all(got[7, [0] + list(range(2, H))] == 0)
+    q, k, v = b.f64()
+    for t in [0, 7, b.rows - 1] + list(r.integers(0, b.rows, size=25)):
+        s = int(np.searchsorted(b.cu_q, t, side="right")) - 1
+        k0, k1 = b.cu_k[s], b.cu_k[s + 1]
+        one = np.array([0, 1]), np.array([0, k1 - k0])
+        want, tol = attend64(q[t:t + 1], k[k0:k1], v[k0:k1], blocks[t:t + 1], *one, block)
+        if kind != "fp32":
+            tol = tol + 2.0 ** -9 * np.abs(v).max()
+        assert np.all(np.abs(got[t] - want[0]) <= tol[0] + 2 * HALF_STEP[kind] * np.abs(want[0])), t
+    np.testing.assert_array_equal(b.attend(blocks, top), b.attend(blocks, top))
+
+
 def selected(b, top):
     q, k, _ = b.f64()
     return select64(q, means64(k, b.cu_k, b.block).astype(np.float32), b.cu_q, b.cb, top)
