@@ -46,6 +46,7 @@ struct GroupedWork {
   int token0 = 0, tokens = 0;  // the tokens in hand
   Divisor by_top, by_heads;
   int head_entries = 0;        // entries of a key head, counting or not
+  int tile_entries = 0;        // most entries of a tile
   int group_heads = 0;         // key heads that are attended to together
   int group_tiles = 0;         // most tiles of such a group
   int* counts = nullptr;       // [cells] entries
@@ -671,7 +672,7 @@ __global__ __launch_bounds__(512) void attention_rows_kernel(BlockAttnArgs p, Se
 
 // ----------------------------------------------- attention, block by block
 // Many rows: the lists are turned round. Every cell (key head, block) gets the
-// entries that list it, and a workgroup multiplies 128 of them with the cell's
+// entries that list it, and a workgroup multiplies 512 of them with the cell's
 // keys and values on the matrix cores, however few neighbours share a block;
 // each entry's part (maximum, sum, weighted values) is written down, a
 // workgroup's together, and a last pass gathers the parts of a row in the order
@@ -681,7 +682,8 @@ __global__ __launch_bounds__(512) void attention_rows_kernel(BlockAttnArgs p, Se
 // An entry is (token - token0, head, list index) as one number; cells are
 // numbered key head first.
 constexpr int kCountThreads = 256, kCountPer = 16, kCountEntries = kCountThreads * kCountPer, kCountBlocks = 8192;
-constexpr int kTileEntries = 512;
+// A workgroup's entries: 512 where that fills the CUs twice, else 128.
+constexpr int kTileEntries = 512, kSmallTileEntries = 128;
 
 // The entries of one workgroup of the two list kernels: one head, and as many
 // tokens as give kCountEntries entries (one token where it has more).
@@ -768,7 +770,7 @@ __global__ __launch_bounds__(kPlaceThreads) void place_cells_kernel(BlockAttnArg
   __shared__ int sums[2][kPlaceThreads / 64];
   __shared__ int base;
   const int hk = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = hk / g.group_heads;
-  auto cell_tiles = [](int n) { return (n + kTileEntries - 1) / kTileEntries; };
+  auto cell_tiles = [&](int n) { return (n + g.tile_entries - 1) / g.tile_entries; };
   int mine = 0;
   for (int b = threadIdx.x; b < p.num_blocks; b += kPlaceThreads) mine += cell_tiles(g.counts[hk * p.num_blocks + b]);
 #pragma unroll
@@ -807,7 +809,7 @@ __global__ __launch_bounds__(kPlaceThreads) void place_cells_kernel(BlockAttnArg
     }
     if (n) g.first[c] = at;
     for (int i = 0; i < tiles; ++i)
-      g.tiles[tile + i] = make_int4(c, at + i * kTileEntries, min(kTileEntries, n - i * kTileEntries), 0);
+      g.tiles[tile + i] = make_int4(c, at + i * g.tile_entries, min(g.tile_entries, n - i * g.tile_entries), 0);
     __syncthreads();
   }
 }
@@ -837,7 +839,7 @@ __global__ __launch_bounds__(kCountThreads) void scatter_entries_kernel(BlockAtt
     }
 }
 
-// One workgroup per tile of up to 512 entries of a cell, 32 at a time to a wave.
+// One workgroup per tile of a cell's entries, 32 at a time to a wave.
 // Keys and values come 64 at a time through LDS as fp16 (hi and lo planes for
 // fp32 tensors), multiplied by powers of two that bring each 64 x dim tile's
 // largest to [2^14, 2^15), and a row of q likewise: full precision at every
@@ -1235,7 +1237,7 @@ int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
 GroupedWork grouped_layout(const BlockAttnArgs& p, const BlockAttnPlan& plan, char* base, size_t* bytes) {
   const size_t cells = static_cast<size_t>(p.num_blocks) * p.kv_heads;
   const size_t entries = static_cast<size_t>(plan.tokens) * p.heads * p.top, head_entries = entries / p.kv_heads;
-  const size_t head_tiles = head_entries / kTileEntries + std::min<size_t>(p.num_blocks, head_entries);
+  const size_t head_tiles = head_entries / plan.tile_entries + std::min<size_t>(p.num_blocks, head_entries);
   const int groups = (p.kv_heads + plan.kv_heads - 1) / plan.kv_heads;
   const size_t parts = head_entries * plan.kv_heads;
   GroupedWork g;
@@ -1248,6 +1250,7 @@ GroupedWork grouped_layout(const BlockAttnArgs& p, const BlockAttnPlan& plan, ch
   g.by_top = Divisor(p.top);
   g.by_heads = Divisor(p.heads);
   g.head_entries = static_cast<int>(head_entries);
+  g.tile_entries = plan.tile_entries;
   g.group_heads = plan.kv_heads;
   g.group_tiles = static_cast<int>(head_tiles * plan.kv_heads);
   g.counts = reinterpret_cast<int*>(take((cells + groups) * 4));
@@ -1352,17 +1355,20 @@ BlockAttnPlan attention_blocks_plan(const BlockAttnArgs& p, const int* cu_q, con
   plan.waves = std::max(1, std::min(8, most));
   if (cells == 0 || cells > 0x3fffffff || entries == 0.0) return plan;
   // Both forms' time in us, as measured over 4 to 768 queries of 8 to 40 heads: row
-  // by row 5 and every entry's keys and values at 7.5 TB/s (from L2); block by block
-  // 24 (six launches), 7.5e-3 for every 32 KB that a workgroup stages and 0.25e-3
-  // for every 32 KB of keys and values that an entry meets in LDS. 20 heads of 64,
-  // fp32, 64 queries over their one block each: 9 and 25; 256 over 4: 80 and 33; 16
-  // over 16 of 250: 45 and 48; 100 over 16 of 250: 181 and 66.
-  const double entry_bytes = keys / entries * p.head_dim * 2 * (type == kTypeF32 ? 4 : 2), unit = entry_bytes / 32768.0;
+  // by row 5 and every entry's keys and values, of 64 keys at least, at 9.5 TB/s
+  // (from L2); block by block 24 (six launches), 7.5e-3 for every 32 KB that a
+  // workgroup stages and 0.25e-3 for every 32 KB of keys and values that an entry
+  // meets in LDS. 20 heads of 64, fp32: 64 queries over their one block each 9 and
+  // 25, 192 over 3 57 and 28, 16 over 16 of 250 45 and 49, 100 over 16 of 250 182
+  // and 65; half precision: 128 over 2 14 and 26.
+  const double row_bytes = p.head_dim * 2.0 * (type == kTypeF32 ? 4 : 2);  // a key and its value
+  const double unit = keys / entries * row_bytes / 32768.0;
   const double hit = cells * (1.0 - std::exp(-entries / cells));
-  const double rows_us = 5.0 + entries * entry_bytes / 7.5e6;
+  const double rows_us = 5.0 + entries * std::max(keys / entries, 64.0) * row_bytes / 9.5e6;
   const double cells_us = 24.0 + (hit + entries / kTileEntries) * 7.5e-3 * unit + entries * 0.25e-3 * unit;
   plan.grouped = cells_us < rows_us;
   if (!plan.grouped) return plan;
+  plan.tile_entries = hit + entries / kTileEntries >= 2.0 * device_cus() ? kTileEntries : kSmallTileEntries;
   // Entry numbers are 32-bit, and lists of 2^26 entries take half a gigabyte.
   plan.tokens = static_cast<int>(std::min<size_t>(p.rows, std::max<size_t>(1, (size_t{1} << 26) / row_entries)));
   const size_t head_bytes =

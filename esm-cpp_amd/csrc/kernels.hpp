@@ -421,7 +421,7 @@ hipError_t launch_select_blocks(const BlockAttnArgs& p, const SeqTable& t, const
 struct BlockAttnPlan {
   bool grouped = false;
   int waves = 1;  // row by row
-  int tokens = 0, kv_heads = 0;
+  int tokens = 0, kv_heads = 0, tile_entries = 0;
   size_t scratch_bytes = 0;
 };
 BlockAttnPlan attention_blocks_plan(const BlockAttnArgs& p, const int* cu_q, const int* cu_k, int batch, int type);
