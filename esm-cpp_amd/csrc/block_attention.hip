@@ -30,9 +30,8 @@ constexpr size_t kPartBytes = size_t{160} << 20;
 // (floor(n m / 2^32) + n) / 2^s (Granlund and Montgomery, 1994).
 struct Divisor {
   uint32_t mul = 0, shift = 0;
-  int d = 1;
   Divisor() = default;
-  explicit Divisor(int by) : d(by) {
+  explicit Divisor(int by) {
     while ((uint64_t{1} << shift) < static_cast<uint64_t>(by)) ++shift;
     mul = static_cast<uint32_t>(((uint64_t{1} << 32) * ((uint64_t{1} << shift) - by)) / by + 1);
   }
@@ -344,7 +343,7 @@ __global__ __launch_bounds__(1024) void select_rows_kernel(BlockAttnArgs p, SeqT
     // Keys 1 .. 2^30 over the row's range where that is finite, else the ordered
     // bits; 0 past the last block. Both keep the order of the scores.
     const float range = most - least;
-    const bool even = range > 1e-30f && range < INFINITY;
+    const bool even = range > 1e-28f && range < INFINITY;  // unit is finite
     const float unit = even ? 1073741696.0f / range : 0.0f;
     uint32_t k4[8][4];
 #pragma unroll
@@ -470,10 +469,12 @@ __device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) {
 }
 
 // The exponent e for which amax * 2^e lies in [2^14, 2^15), where fp16 holds
-// hi + lo parts to 22 bits down to 2^-39 of the largest; within -60 .. 60, so
-// that the inverse of a product of two such scales is a normal number.
-__device__ __forceinline__ int scale_exponent(float amax) {
-  return amax > 0.0f ? max(-60, min(60, 15 - __builtin_amdgcn_frexp_expf(amax))) : 0;
+// hi + lo parts to 22 bits down to 2^-39 of the largest; within -most .. most. Q
+// and K are held to 60, so that the inverse of their scales' product is a normal
+// number (a score's error is absolute: rows below 2^-45 only matter to keys above
+// 2^20 and the other way round), V to 120.
+__device__ __forceinline__ int scale_exponent(float amax, int most = 60) {
+  return amax > 0.0f ? max(-most, min(most, 15 - __builtin_amdgcn_frexp_expf(amax))) : 0;
 }
 
 // Eight consecutive elements as fp32.
@@ -714,7 +715,7 @@ __global__ __launch_bounds__(kCountThreads) void count_entries_kernel(BlockAttnA
     const int e = i - tok[u] * p.top;
     const int* at = lists + static_cast<size_t>(tok[u]) * p.heads * p.top + e;
     block[u] = *at;
-    before[u] = e > 0 ? at[-1] : 0x80000000;
+    before[u] = at[e > 0 ? -1 : 0];
   }
   for (int i = threadIdx.x; lds && i < p.num_blocks; i += kCountThreads) hist[i] = 0;
   for (int i = threadIdx.x, n = g.by_top(r.entries); i < n; i += kCountThreads) unsorted[i] = 0;
@@ -723,9 +724,9 @@ __global__ __launch_bounds__(kCountThreads) void count_entries_kernel(BlockAttnA
   // no repeats.
 #pragma unroll
   for (int u = 0; u < kCountPer; ++u) {
-    if (u * kCountThreads + static_cast<int>(threadIdx.x) >= r.entries) block[u] = -1;
-    if (block[u] >= 0 && before[u] != static_cast<int>(0x80000000) && (before[u] < 0 || block[u] <= before[u]))
-      unsorted[tok[u]] = 1;
+    const int i = u * kCountThreads + threadIdx.x;
+    if (i >= r.entries) block[u] = -1;
+    if (i - tok[u] * p.top > 0 && block[u] >= 0 && (before[u] < 0 || block[u] <= before[u])) unsorted[tok[u]] = 1;
   }
   __syncthreads();
   int place[kCountPer];
@@ -842,7 +843,7 @@ __global__ __launch_bounds__(kCountThreads) void scatter_entries_kernel(BlockAtt
 // One workgroup per tile of a cell's entries, 32 at a time to a wave.
 // Keys and values come 64 at a time through LDS as fp16 (hi and lo planes for
 // fp32 tensors), multiplied by powers of two that bring each 64 x dim tile's
-// largest to [2^14, 2^15), and a row of q likewise: full precision at every
+// largest to [2^14, 2^15), and a row of q likewise: full precision whatever their
 // magnitude. Blocks of at most 64 keys are staged once, and the waves then walk
 // the tile's entries on their own, the next ones' queries on their way. S^T =
 // K Q^T leaves a lane the scores of one query with keys 4 lg .. + 4 of every 16,
@@ -905,7 +906,7 @@ __global__ __launch_bounds__(256) void attention_cells_kernel(BlockAttnArgs p, S
     }
     __syncthreads();  // also: the last 64 keys' reads are done
     ke = scale_exponent(fmaxf(fmaxf(tile_max[0][0], tile_max[0][1]), fmaxf(tile_max[0][2], tile_max[0][3])));
-    ve = scale_exponent(fmaxf(fmaxf(tile_max[1][0], tile_max[1][1]), fmaxf(tile_max[1][2], tile_max[1][3])));
+    ve = scale_exponent(fmaxf(fmaxf(tile_max[1][0], tile_max[1][1]), fmaxf(tile_max[1][2], tile_max[1][3])), 120);
     const float kmul = __builtin_amdgcn_ldexpf(1.0f, ke), vmul = __builtin_amdgcn_ldexpf(1.0f, ve);
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {

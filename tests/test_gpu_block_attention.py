@@ -233,6 +233,44 @@ def test_large_scores_and_far_apart_values(dev, rows):
     b.check(selected(b, 4))
 
 
+@pytest.mark.parametrize("rows", [2, 900])
+def test_repeats_behind_negative_entries(dev, rows):
+    """A repeat is one whatever stands between: the most negative number too."""
+    b = Batch(dev, "fp32", [rows], [300], 4, 4, 64, 32, seed=7)
+    for middle in (-1, -2 ** 31):
+        for j in (0, 3):
+            blocks = np.full((rows, 4, 4), -1, np.int32)
+            blocks[:, :, 0], blocks[:, :, 1], blocks[:, :, 2], blocks[:, :, 3] = j, middle, j, 7
+            once = blocks.copy()
+            once[:, :, 2] = -1
+            np.testing.assert_array_equal(b.attend(blocks, 4), b.attend(once, 4))
+
+
+@pytest.mark.parametrize("rows", [3, 700])
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e25])
+def test_values_of_any_magnitude(dev, rows, scale):
+    """The output is linear in V: scaling it by a power of two scales the result."""
+    b = Batch(dev, "fp32", [rows], [400], 4, 4, 64, 64, seed=15)
+    blocks = rng(3).integers(0, 7, size=(rows, 4, 3)).astype(np.int32)
+    want = b.attend(blocks, 3)
+    by = np.float32(2.0 ** round(np.log2(scale)))
+    b.v = b.v * by
+    np.testing.assert_allclose(b.attend(blocks, 3), want * by, rtol=2e-6, atol=2e-6 * float(by))
+
+
+@pytest.mark.parametrize("scale", [1e-36, 1e-30, 1e-20, 1e15, 1e18])
+def test_selection_of_any_magnitude(dev, scale):
+    """Scores from below fp32's smallest to near its largest numbers."""
+    r = rng(5)
+    rows, H, dim, nb, top, block = 40, 2, 32, 70, 9, 16
+    cu_q, cu_k = cu_from_lengths([rows]), cu_from_lengths([nb * block])
+    q = (r.standard_normal((rows, H, dim)) * scale).astype(np.float32)
+    m = (r.standard_normal((nb, H, dim)) * min(scale, 1e4)).astype(np.float32)
+    out = dev.empty((rows, H, top), np.int32)
+    dev.attention_select_blocks(dev.array(q), dev.array(m), cu_q, cu_k, H, H, dim, block, top, out)
+    np.testing.assert_array_equal(out.numpy(), select64(q.astype(np.float64), m, cu_q, eg.key_blocks(cu_k, block), top))
+
+
 @pytest.mark.parametrize("rows", [2, 130])
 @pytest.mark.parametrize("kind", list(TYPES))
 def test_what_is_not_listed_is_not_read(dev, kind, rows):
