@@ -362,6 +362,7 @@ struct LinearI4Plan {
   enum Form { kRows, kMid, kGemm } form = kRows;
   int col_tiles = 1;  // kRows: 16-column tiles per workgroup
   int waves = 1;      // kRows, kMid
+  bool wide = false;  // kMid: larger tiles than 16 x 32
   int chunk = 1;      // kRows: 128-input tiles whose activations are in LDS at a time
   size_t scratch_bytes = 0;
 };

@@ -573,22 +573,28 @@ hipError_t launch_rows(const LinearI4Args& p, const LinearI4Plan& plan, hipStrea
   const unsigned grid = static_cast<unsigned>((p.N + 16 * NT - 1) / (16 * NT)), block = 64 * plan.waves;
   const size_t row_bytes = static_cast<size_t>(plan.chunk) * (Elem<DT>::kPlanes * 256 + 4) + 16;
   const size_t lds = std::max(p.M * row_bytes, static_cast<size_t>(plan.waves) * NT * 1024);
-#define KERNEL(GJ, _) linear_i4_rows_kernel<DT, NT, GJ><<<grid, block, lds, s>>>(p, plan.chunk)
-  ESM_I4_BY_GROUP(KERNEL, 0);
-#undef KERNEL
+  if (p.group == 64) {
+    linear_i4_rows_kernel<DT, NT, 2><<<grid, block, lds, s>>>(p, plan.chunk);
+  } else if (p.group != 32) {
+    linear_i4_rows_kernel<DT, NT, 4><<<grid, block, lds, s>>>(p, plan.chunk);
+  } else {
+    if constexpr (NT == 1) linear_i4_rows_kernel<DT, 1, 1><<<grid, block, lds, s>>>(p, plan.chunk);
+  }
   return hipGetLastError();
 }
 
-template <int DT, int GJ>
+template <int DT, int MT, int NT, int GJ>
 void launch_mid(const LinearI4Args& p, const LinearI4Plan& plan, const uint16_t* planes, const float* inv, int ldp,
                 hipStream_t s) {
-  // Two tiles in flight have to fit the registers.
-  constexpr int MT = 2, NT = Elem<DT>::kPlanes == 2 || GJ == 1 ? 2 : 4;
   const unsigned grid =
       static_cast<unsigned>((p.N + 16 * NT - 1) / (16 * NT)) * ((p.M + 16 * MT - 1) / (16 * MT));
   const size_t lds = static_cast<size_t>(plan.waves) * NT * MT * 1024;
   linear_i4_mid_kernel<DT, MT, NT, GJ><<<grid, 64 * plan.waves, lds, s>>>(p, planes, inv, ldp);
 }
+
+// The wide form's tiles: as large as two of them in flight fit the registers.
+constexpr int wide_rows(bool two_planes, bool group32) { return two_planes && !group32 ? 1 : 2; }
+constexpr int wide_cols(bool group32) { return group32 ? 2 : 4; }
 
 template <int DT>
 hipError_t launch_typed(const LinearI4Args& p, const LinearI4Plan& plan, void* scratch, hipStream_t s) {
@@ -605,7 +611,10 @@ hipError_t launch_typed(const LinearI4Args& p, const LinearI4Plan& plan, void* s
     inv = DT == kTypeF16 ? nullptr : units;
   }
   if (plan.form == LinearI4Plan::kMid) {
-#define KERNEL(GJ, _) launch_mid<DT, GJ>(p, plan, planes, inv, ldp, s)
+#define KERNEL(GJ, _)                                                                                    \
+  plan.wide ? launch_mid<DT, wide_rows(Elem<DT>::kPlanes == 2, GJ == 1), wide_cols(GJ == 1), GJ>(        \
+                  p, plan, planes, inv, ldp, s)                                                          \
+            : launch_mid<DT, 1, 2, GJ>(p, plan, planes, inv, ldp, s)
     ESM_I4_BY_GROUP(KERNEL, 0);
 #undef KERNEL
   } else {
@@ -623,9 +632,13 @@ hipError_t launch_typed(const LinearI4Args& p, const LinearI4Plan& plan, void* s
 LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type) {
   LinearI4Plan plan;
   const size_t tiles_n = (static_cast<size_t>(p.N) + kTileN - 1) / kTileN, cus = std::max(1, device_cus());
-  if (p.M <= 16) {
+  // Rows that the kernels can read in place need no scratch, and no launch that
+  // splits them: then 9 rows are already better off without LDS (16 fp16 rows of
+  // 1,280 x 5,120 10.4 us split in the kernel, 8.6 read in place).
+  const bool in_place = type == kTypeF16 && p.vec_a && p.K % kTileK == 0;
+  if (p.M <= (in_place ? 8 : 16)) {
     plan.form = LinearI4Plan::kRows;
-    plan.col_tiles = tiles_n >= 2 * cus ? 2 : 1;
+    plan.col_tiles = tiles_n >= 2 * cus && p.group != 32 ? 2 : 1;  // two with four groups a tile spill
     // As many waves as give each the same number of tiles, at most 10, and as many
     // of the waves' tiles at a time as keep the activations in 60 KB of LDS.
     const int rounds = (p.tiles_k + 9) / 10;
@@ -635,27 +648,30 @@ LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type) {
     if (plan.chunk == 0) plan.chunk = plan.waves = std::max(1, fit);
     return plan;
   }
-  // Rows that the kernels can read in place need no scratch.
-  const bool in_place = type == kTypeF16 && p.vec_a && p.K % kTileK == 0;
   const int ldp = in_place ? p.lda : p.tiles_k * kTileK;
-  // Both kernels' time on an idle device, in us, as measured over 17 to 2,048 rows
-  // of 1,280 x 1,280, 5,120 x 1,280, 1,280 x 5,120 and 10,240 x 2,560: small tiles
-  // take 3.0 (fp32: 3.9) for each 128-input tile of a wave in each round of one
-  // workgroup per CU; a GEMM workgroup 10 and 0.6 (0.97) per 64 inputs while it has
-  // a CU to itself, 1.4 times that where two share one, and rounds of those. So 256
-  // fp32 rows of 5,120 x 1,280 are a GEMM (32 us, small tiles 41) and 512 of
-  // 1,280 x 5,120 small tiles (72, GEMM 90).
-  const bool two = type == kTypeF32;
-  const int mid_cols = 16 * (two || p.group == 32 ? 2 : 4);
-  const double mid_wgs = static_cast<double>((p.M + 31) / 32) * ((static_cast<size_t>(p.N) + mid_cols - 1) / mid_cols);
-  const double gemm_wgs = static_cast<double>((static_cast<size_t>(p.M) + kGemmM - 1) / kGemmM) *
-                          static_cast<double>((static_cast<size_t>(p.N) + kGemmN - 1) / kGemmN);
-  const double mid_us = (two ? 3.9 : 3.0) * ((p.tiles_k + 7) / 8) * std::ceil(mid_wgs / cus);
+  // The kernels' time on an idle device, in us, as measured over 17 to 2,048 rows
+  // of 1,280 x 1,280, 5,120 x 1,280, 1,280 x 5,120 and 10,240 x 2,560. Small tiles
+  // take a time for each 128-input tile of a wave in each round of one workgroup per
+  // CU: 16 x 32 ones 1.75 (fp32: 2.9) in the one round that they are used for, wide
+  // ones 3.0 (3.1, with groups of 32 3.9). A GEMM workgroup takes 10 and 0.6 (0.97)
+  // per 64 inputs while it has a CU to itself, 1.4 times that where two share one,
+  // and rounds of those. So 67 fp16 rows of 1,280 x 5,120 take 16 x 32 tiles (9 us,
+  // wide ones 15) and 301 wide ones (16, the others 22); 192 fp32 rows of 5,120 x
+  // 1,280 take wide tiles (25, as a GEMM 31), 512 of 1,280 x 5,120 too (50, as a GEMM
+  // 90), and 768 of 5,120 x 1,280 are a GEMM (38, 112 in 32 x 32 tiles).
+  const bool two = type == kTypeF32, g32 = p.group == 32;
+  auto tiles = [](int n, int by) { return (static_cast<double>(n) + by - 1) / by; };
+  const auto wgs = [&](int rows, int cols) { return std::floor(tiles(p.M, rows)) * std::floor(tiles(p.N, cols)); };
+  const double iterations = (p.tiles_k + 7) / 8;
+  const double wide_wgs = wgs(16 * wide_rows(two, g32), 16 * wide_cols(g32)), gemm_wgs = wgs(kGemmM, kGemmN);
+  const double narrow_us = wgs(16, 32) <= cus ? (two ? 2.9 : 1.75) * iterations : 1e30;
+  const double wide_us = (two ? (g32 ? 3.9 : 3.1) : 3.0) * iterations * std::ceil(wide_wgs / cus);
   const double gemm_us = (10.0 + (two ? 0.97 : 0.6) * 2 * p.tiles_k) *
                          (gemm_wgs <= cus ? 1.0 : 1.4 * std::max(1.0, gemm_wgs / (2.0 * cus)));
   // A GEMM tile's 64 rows are 32-bit offsets apart, and its grid is one number.
   const bool gemm_ok = ldp < (1 << 23) && gemm_wgs < 2e9;
-  plan.form = gemm_ok && gemm_us < mid_us ? LinearI4Plan::kGemm : LinearI4Plan::kMid;
+  plan.wide = wide_us < narrow_us;
+  plan.form = gemm_ok && gemm_us < std::min(narrow_us, wide_us) ? LinearI4Plan::kGemm : LinearI4Plan::kMid;
   plan.waves = std::min(8, p.tiles_k);
   if (!in_place)
     plan.scratch_bytes =
