@@ -355,9 +355,9 @@ struct LinearI4Args {
   int tiles_k = 0;  // ceil(K / 128)
   bool vec_a = false;  // A's rows start at 16-byte addresses
 };
-// How linear_i4 runs: up to 16 rows with the activations split in the kernel, or
-// on activations split into scratch beforehand, in small tiles with the inputs
-// spread over the waves or as a GEMM.
+// How linear_i4 runs: few rows (up to 16, or 8 that need no splitting) with the
+// activations split in the kernel, or on activations split into scratch
+// beforehand, in small tiles with the inputs spread over the waves or as a GEMM.
 struct LinearI4Plan {
   enum Form { kRows, kMid, kGemm } form = kRows;
   int col_tiles = 1;  // kRows: 16-column tiles per workgroup

@@ -4,10 +4,11 @@
 //
 // A code is an fp16 number as it stands, so the products run on fp16 MFMA with
 // the weight operand exact: for fp16 activations directly, for bf16 ones (8
-// significant bits) after a power of two per row and 128 inputs that brings the
-// largest of them to [2^14, 2^15), and for fp32 ones as hi + lo fp16 parts (22
-// significant bits) of the same scaled value, two MFMAs per product. A group's
-// sum leaves the matrix cores before it is multiplied by its scale (and by the
+// significant bits) after a power of two that brings the largest of a row (of 128
+// of its inputs, in the kernel for few rows) to [2^14, 2^15), and for fp32 ones as
+// hi + lo fp16 parts (22 significant bits) of the same scaled value, two MFMAs per
+// product. What lies far below the largest is off by half of fp16's smallest step
+// at most, 2^-39 of the largest. A group's sum leaves the matrix cores before it is multiplied by its scale (and by the
 // power of two's inverse): one fused multiply-add per output, group and row.
 //
 // Weights lie in tiles of 16 outputs x 128 inputs, 1 KB, in the order of the
