@@ -31,6 +31,9 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTileN = 16, kTileK = 128;
 
+// Elements from one plane of split activations to the next: rows in sixteens.
+__host__ __device__ inline size_t plane_elems(int M, int ldp) { return (static_cast<size_t>(M) + 15) / 16 * 16 * ldp; }
+
 // Eight codes of one dword as fp16.
 __device__ __forceinline__ f16x8 unpack_codes(uint32_t w) {
   const f16x2 k1032 = {static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)};
@@ -252,18 +255,24 @@ __global__ __launch_bounds__(1024) void linear_i4_rows_kernel(LinearI4Args p, in
 
 // ------------------------------------------------------------- many rows
 // Activations as the matrix cores take them, written once for every column tile:
-// fp16 planes [planes][M][ldp] (hi, and lo for fp32), zeros past K, a row scaled
-// by the power of two that brings its largest to [2^14, 2^15), the power's inverse
-// in inv; fp16 rows as they are, where their alignment or length keeps the
-// kernels from reading them in place. One workgroup per row.
-template <int DT>
+// fp16 planes (hi, and lo for fp32) of M rows, rounded up to 16, of ldp inputs,
+// zeros past K, a row scaled by the power of two that brings its largest to
+// [2^14, 2^15), the power's inverse in inv; fp16 rows as they are, where their
+// alignment or length keeps the kernels from reading them in place. One workgroup
+// per row. Row after row for the GEMM; for the small tiles (TILED) 16 rows x 32
+// inputs after each other in the lanes' order, which the kernel loads in whole
+// kilobytes (row by row, four neighbouring lanes' 16 bytes lie in four rows and
+// take four accesses). The 16 rows of a tile are then one XCD's, whose L2 joins
+// their pieces.
+template <int DT, bool TILED>
 __global__ __launch_bounds__(256) void linear_i4_split_kernel(LinearI4Args p, uint16_t* planes, float* inv, int ldp) {
   using T = typename Elem<DT>::T;
   __shared__ float part[4];
-  const int m = blockIdx.x;
+  const int m = TILED ? (blockIdx.x % 8 + blockIdx.x / 128 * 8) * 16 + blockIdx.x / 8 % 16 : blockIdx.x;
+  if (m >= p.M) return;
   const T* row = static_cast<const T*>(p.A) + static_cast<size_t>(m) * p.lda;
-  uint16_t* hi = planes + static_cast<size_t>(m) * ldp;
-  uint16_t* lo = hi + static_cast<size_t>(p.M) * ldp;
+  uint16_t* hi = planes + (TILED ? static_cast<size_t>(m / 16) * 16 * ldp + m % 16 * 8 : static_cast<size_t>(m) * ldp);
+  uint16_t* lo = hi + plane_elems(p.M, ldp);
   float mul = 1.0f;
   if constexpr (DT != kTypeF16) {
     float amax = 0.0f;
@@ -293,18 +302,22 @@ __global__ __launch_bounds__(256) void linear_i4_split_kernel(LinearI4Args p, ui
       h[i] = static_cast<_Float16>(v);
       l[i] = static_cast<_Float16>(fabsf(v) < INFINITY ? v - static_cast<float>(h[i]) : 0.0f);
     }
-    *reinterpret_cast<f16x8*>(hi + k) = h;
-    if constexpr (Elem<DT>::kPlanes == 2) *reinterpret_cast<f16x8*>(lo + k) = l;
+    const size_t at = TILED ? static_cast<size_t>(k) * 16 : k;  // eight inputs of 16 rows: 128 elements
+    *reinterpret_cast<f16x8*>(hi + at) = h;
+    if constexpr (Elem<DT>::kPlanes == 2) *reinterpret_cast<f16x8*>(lo + at) = l;
   }
 }
 
 // 16 MT rows x 16 NT outputs per workgroup, for grids that larger tiles would
-// leave empty: the waves take the 128-input tiles in turn, each straight from
-// memory into its operand registers while the one before is computed, and add up
-// through LDS.
+// leave empty: the waves take the 128-input tiles in turn, straight from memory
+// into their operand registers, and add up through LDS. 16 x 32 tiles wait for
+// each tile's loads and leave the CU to two or three other workgroups meanwhile
+// (67 fp32 rows of 3,840 x 1,280 11.1 us a call, 14.5 with the next tile's loads in
+// flight and one workgroup a CU); 32 x 64 ones (one plane only) have those in flight.
+// in_place: planes are the caller's fp16 rows, not the split kernel's.
 template <int DT, int MT, int NT, int GJ>
-__global__ __launch_bounds__(512) void linear_i4_mid_kernel(LinearI4Args p, const uint16_t* planes, const float* inv,
-                                                            int ldp) {
+__global__ __launch_bounds__(512, NT == 2 ? 4 : 2) void linear_i4_mid_kernel(
+    LinearI4Args p, const uint16_t* planes, const float* inv, int ldp, bool in_place) {
   using T = typename Elem<DT>::T;
   constexpr int PL = Elem<DT>::kPlanes;
   extern __shared__ float red[];
@@ -312,11 +325,15 @@ __global__ __launch_bounds__(512) void linear_i4_mid_kernel(LinearI4Args p, cons
   const int lr = lane & 15, kq = lane >> 4;
   const int cols = (p.N + 16 * NT - 1) / (16 * NT), tiles_n = (p.N + kTileN - 1) / kTileN;
   const int tn0 = blockIdx.x % cols * NT, m0 = blockIdx.x / cols * (16 * MT);
+  constexpr bool kAhead = NT > 2;
+  const bool rowwise = DT == kTypeF16 && in_place;
   const uint16_t* rows[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
-    rows[mt] = planes + static_cast<size_t>(min(m0 + 16 * mt + lr, p.M - 1)) * ldp + 8 * kq;
-  const size_t plane = static_cast<size_t>(p.M) * ldp;
+    rows[mt] = planes + (rowwise ? static_cast<size_t>(min(m0 + 16 * mt + lr, p.M - 1)) * ldp + 8 * kq
+                                 : static_cast<size_t>(min(m0 / 16 + mt, (p.M - 1) / 16)) * 16 * ldp + 8 * lane);
+  const size_t step = rowwise ? 32 : 512;  // elements from 32 inputs to the next 32
+  const size_t plane = plane_elems(p.M, ldp);
   struct Tile {
     u32x4 w[NT];
     f32x4 s[NT][4 / GJ];
@@ -339,7 +356,7 @@ __global__ __launch_bounds__(512) void linear_i4_mid_kernel(LinearI4Args p, cons
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int pl = 0; pl < PL; ++pl)
-          t.a[mt][j][pl] = *reinterpret_cast<const f16x8*>(rows[mt] + pl * plane + kt * kTileK + 32 * j);
+          t.a[mt][j][pl] = *reinterpret_cast<const f16x8*>(rows[mt] + pl * plane + (kt * 4 + j) * step);
   };
   f32x4 total[NT][MT];
 #pragma unroll
@@ -347,10 +364,11 @@ __global__ __launch_bounds__(512) void linear_i4_mid_kernel(LinearI4Args p, cons
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) total[nt][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
   Tile next;
-  if (wave < p.tiles_k) load(wave, next);
+  if (kAhead && wave < p.tiles_k) load(wave, next);
   for (int kt = wave; kt < p.tiles_k; kt += waves) {
+    if (!kAhead) load(kt, next);
     const Tile t = next;
-    if (kt + waves < p.tiles_k) load(kt + waves, next);
+    if (kAhead && kt + waves < p.tiles_k) load(kt + waves, next);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       f32x4 acc[MT];
@@ -423,11 +441,11 @@ __global__ __launch_bounds__(256) void linear_i4_gemm_kernel(LinearI4Args p, con
     const int r = wave * 16 + i * 8 + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
     off[i] = static_cast<uint32_t>(min(r, p.M - 1 - m0)) * static_cast<uint32_t>(ldp * 2) + c * 16;
   }
-  const size_t plane_elems = PL == 2 ? static_cast<size_t>(p.M) * ldp : 0;
+  const size_t plane = PL == 2 ? plane_elems(p.M, ldp) : 0;
   auto load_stage = [&](int k0, int buf) {
 #pragma unroll
     for (int pl = 0; pl < PL; ++pl) {
-      const uint16_t* base = planes + pl * plane_elems + static_cast<size_t>(m0) * ldp + k0;
+      const uint16_t* base = planes + pl * plane + static_cast<size_t>(m0) * ldp + k0;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         lds_dma16(base, off[i], lds0 + buf * (PL * kPlaneBytes) + pl * kPlaneBytes + (wave * 16 + i * 8) * 128);
@@ -590,12 +608,8 @@ void launch_mid(const LinearI4Args& p, const LinearI4Plan& plan, const uint16_t*
   const unsigned grid =
       static_cast<unsigned>((p.N + 16 * NT - 1) / (16 * NT)) * ((p.M + 16 * MT - 1) / (16 * MT));
   const size_t lds = static_cast<size_t>(plan.waves) * NT * MT * 1024;
-  linear_i4_mid_kernel<DT, MT, NT, GJ><<<grid, 64 * plan.waves, lds, s>>>(p, planes, inv, ldp);
+  linear_i4_mid_kernel<DT, MT, NT, GJ><<<grid, 64 * plan.waves, lds, s>>>(p, planes, inv, ldp, plan.scratch_bytes == 0);
 }
-
-// The wide form's tiles: as large as two of them in flight fit the registers.
-constexpr int wide_rows(bool two_planes, bool group32) { return two_planes && !group32 ? 1 : 2; }
-constexpr int wide_cols(bool group32) { return group32 ? 2 : 4; }
 
 template <int DT>
 hipError_t launch_typed(const LinearI4Args& p, const LinearI4Plan& plan, void* scratch, hipStream_t s) {
@@ -606,18 +620,25 @@ hipError_t launch_typed(const LinearI4Args& p, const LinearI4Plan& plan, void* s
   if (plan.scratch_bytes) {
     ldp = p.tiles_k * kTileK;
     auto* to = static_cast<uint16_t*>(scratch);
-    auto* units = reinterpret_cast<float*>(to + static_cast<size_t>(Elem<DT>::kPlanes) * p.M * ldp);
-    linear_i4_split_kernel<DT><<<p.M, 256, 0, s>>>(p, to, units, ldp);
+    auto* units = reinterpret_cast<float*>(to + Elem<DT>::kPlanes * plane_elems(p.M, ldp));
+    if (plan.form == LinearI4Plan::kMid)
+      linear_i4_split_kernel<DT, true><<<(p.M + 127) / 128 * 128, 256, 0, s>>>(p, to, units, ldp);
+    else
+      linear_i4_split_kernel<DT, false><<<p.M, 256, 0, s>>>(p, to, units, ldp);
     planes = to;
     inv = DT == kTypeF16 ? nullptr : units;
   }
   if (plan.form == LinearI4Plan::kMid) {
-#define KERNEL(GJ, _)                                                                                    \
-  plan.wide ? launch_mid<DT, wide_rows(Elem<DT>::kPlanes == 2, GJ == 1), wide_cols(GJ == 1), GJ>(        \
-                  p, plan, planes, inv, ldp, s)                                                          \
-            : launch_mid<DT, 1, 2, GJ>(p, plan, planes, inv, ldp, s)
-    ESM_I4_BY_GROUP(KERNEL, 0);
+    if (!plan.wide) {
+#define KERNEL(GJ, _) launch_mid<DT, 1, 2, GJ>(p, plan, planes, inv, ldp, s)
+      ESM_I4_BY_GROUP(KERNEL, 0);
 #undef KERNEL
+    } else if constexpr (Elem<DT>::kPlanes == 1) {
+      if (p.group == 64)
+        launch_mid<DT, 2, 4, 2>(p, plan, planes, inv, ldp, s);
+      else
+        launch_mid<DT, 2, 4, 4>(p, plan, planes, inv, ldp, s);
+    }
   } else {
     const unsigned grid =
         static_cast<unsigned>((p.M + kGemmM - 1) / kGemmM) * static_cast<unsigned>((p.N + kGemmN - 1) / kGemmN);
@@ -650,33 +671,34 @@ LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type) {
     return plan;
   }
   const int ldp = in_place ? p.lda : p.tiles_k * kTileK;
-  // The kernels' time on an idle device, in us, as measured over 17 to 2,048 rows
-  // of 1,280 x 1,280, 5,120 x 1,280, 1,280 x 5,120 and 10,240 x 2,560. Small tiles
-  // take a time for each 128-input tile of a wave in each round of one workgroup per
-  // CU: 16 x 32 ones 1.75 (fp32: 2.9) in the one round that they are used for, wide
-  // ones 3.0 (3.1, with groups of 32 3.9). A GEMM workgroup takes 10 and 0.6 (0.97)
-  // per 64 inputs while it has a CU to itself, 1.4 times that where two share one,
-  // and rounds of those. So 67 fp16 rows of 1,280 x 5,120 take 16 x 32 tiles (9 us,
-  // wide ones 15) and 301 wide ones (16, the others 22); 192 fp32 rows of 5,120 x
-  // 1,280 take wide tiles (25, as a GEMM 31), 512 of 1,280 x 5,120 too (50, as a GEMM
-  // 90), and 768 of 5,120 x 1,280 are a GEMM (38, 112 in 32 x 32 tiles).
+  // The call's time on an idle device, in us, as measured over 17 to 512 rows of
+  // 1,280 x 1,280, 3,840 x 1,280, 5,120 x 1,280, 1,280 x 5,120 and 10,240 x 2,560,
+  // the rows' split left out: small tiles 1 for each 128-input tile of a wave and, as
+  // the CUs hold two or three, 0.15 (two planes and groups of 32: 0.2) for each of a
+  // CU's; wide ones 3 for each of a wave's in each round of one workgroup per CU; a
+  // GEMM workgroup 10 and 0.6 (two planes 0.97, groups of 32 0.4 more) per 64 inputs
+  // while it has a CU to itself, 1.4 times that where two share one, and rounds of
+  // those. So 67 fp32 rows of 3,840 x 1,280 take small tiles (11 us, as a GEMM 40),
+  // 256 too (23, 42), 512 of 1,280 x 5,120 as well (40, 90) and 256 of 10,240 x
+  // 2,560 are a GEMM (54, in small tiles 58); 301 fp16 rows of 1,280 x 5,120 take
+  // wide tiles (16, small ones 21, as a GEMM 57).
   const bool two = type == kTypeF32, g32 = p.group == 32;
-  auto tiles = [](int n, int by) { return (static_cast<double>(n) + by - 1) / by; };
+  auto tiles = [](int n, int by) { return (n + by - 1.0) / by; };
   const auto wgs = [&](int rows, int cols) { return std::floor(tiles(p.M, rows)) * std::floor(tiles(p.N, cols)); };
-  const double iterations = (p.tiles_k + 7) / 8;
-  const double wide_wgs = wgs(16 * wide_rows(two, g32), 16 * wide_cols(g32)), gemm_wgs = wgs(kGemmM, kGemmN);
-  const double narrow_us = wgs(16, 32) <= cus ? (two ? 2.9 : 1.75) * iterations : 1e30;
-  const double wide_us = (two ? (g32 ? 3.9 : 3.1) : 3.0) * iterations * std::ceil(wide_wgs / cus);
-  const double gemm_us = (10.0 + (two ? 0.97 : 0.6) * 2 * p.tiles_k) *
+  const int iterations = (p.tiles_k + 7) / 8;
+  const double gemm_wgs = wgs(kGemmM, kGemmN);
+  const double small_us = iterations + (two && g32 ? 0.2 : 0.15) * p.tiles_k * wgs(16, 32) / cus;
+  const double wide_us = two || g32 ? 1e30 : 3.0 * iterations * std::ceil(wgs(32, 64) / cus);
+  const double gemm_us = (10.0 + ((two ? 0.97 : 0.6) + (g32 ? 0.4 : 0.0)) * 2 * p.tiles_k) *
                          (gemm_wgs <= cus ? 1.0 : 1.4 * std::max(1.0, gemm_wgs / (2.0 * cus)));
   // A GEMM tile's 64 rows are 32-bit offsets apart, and its grid is one number.
   const bool gemm_ok = ldp < (1 << 23) && gemm_wgs < 2e9;
-  plan.wide = wide_us < narrow_us;
-  plan.form = gemm_ok && gemm_us < std::min(narrow_us, wide_us) ? LinearI4Plan::kGemm : LinearI4Plan::kMid;
-  plan.waves = std::min(8, p.tiles_k);
+  plan.wide = wide_us < small_us;
+  plan.form = gemm_ok && gemm_us < std::min(small_us, wide_us) ? LinearI4Plan::kGemm : LinearI4Plan::kMid;
+  plan.waves = (p.tiles_k + iterations - 1) / iterations;
   if (!in_place)
     plan.scratch_bytes =
-        static_cast<size_t>(p.M) * (static_cast<size_t>(p.tiles_k) * kTileK * (type == kTypeF32 ? 4 : 2) + 4);
+        plane_elems(p.M, ldp) * (type == kTypeF32 ? 4 : 2) + static_cast<size_t>(p.M) * 4;
   return plan;
 }
 

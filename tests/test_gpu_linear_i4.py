@@ -107,6 +107,14 @@ def test_many_rows_and_columns(dev, kind, M, N, K, group):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("M,N,K,group", [(301, 1290, 5120, 128), (301, 1290, 5000, 128), (291, 1300, 5120, 64),
+                                         (291, 1300, 4999, 64), (100, 3850, 1270, 32)])
+def test_some_rows_of_long_sums(dev, kind, M, N, K, group):
+    """Sizes at which small tiles share the CUs, and 16-bit types take wider ones."""
+    check(dev, kind, M, N, K, group, seed=M + N + K + group)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("offset,pad", [(0, 8), (1, 3)])
 def test_strides_of_many_rows_and_columns(dev, kind, offset, pad):
     M, N, K, group = 650, 5130, 256, 64
