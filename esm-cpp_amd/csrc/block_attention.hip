@@ -112,8 +112,8 @@ __device__ __forceinline__ uint64_t score_key(double s) {
 
 // One workgroup per block and 64 16-byte column pieces: a lane has a piece, a wave
 // every fourth key, eight loads in flight; the waves' 64-bit sums meet in LDS.
-// Bound by the keys' bytes. (A thread per column, one element at a time, took 146
-// us for 61,773 bf16 keys of 20 heads, 158 MB.)
+// Bound by the keys' bytes: 61,773 bf16 keys of 20 heads, 158 MB, in 27 us, at the
+// rate of a large copy. (A thread per column, one element at a time, took 146.)
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void block_means_kernel(BlockAttnArgs p, SeqTable t) {
   using T = typename ElemOf<DT>::T;
@@ -236,8 +236,10 @@ __device__ __forceinline__ double score64(const float* q, const float* m, int di
 // powers of two of the gap there, two instructions per score each). Where that
 // cannot tell the last ones apart, the row is settled with 64-bit scores.
 //
-// One wave per row with 64-bit scores summed lane by lane and a ballot per step
-// took 2.2 ms for 7,930 queries of 20 heads.
+// 7,930 queries of 20 heads over 21 to 65 blocks: 80 us, of it about 13 the fp64
+// products; the threshold's steps on the VALU and their latency at 16 waves a CU are
+// the rest. One wave per row with 64-bit scores summed lane by lane and a ballot per
+// step took 2.2 ms.
 constexpr int kSelBlocks = 960;  // a 16-row tile's keys fit 64 KB of LDS
 
 template <int DT, int DH>
@@ -546,7 +548,9 @@ __device__ __forceinline__ float group_sum(float v) {
 // Few rows: one workgroup per (query, head), a wave per listed block, joined in
 // LDS. The 16-byte pieces of a key lie in LPK neighbouring lanes, 64 / LPK keys
 // to a load. After the loads' products a butterfly over the lanes (each step
-// hands half of the lane's values over) leaves every lane one key's score.
+// hands half of the lane's values over) leaves every lane one key's score. Bound by
+// the launch and three dependent trips to memory (list, keys, values): 3 queries of
+// 20 heads, 16 blocks of 64 keys each, 11 us.
 template <int DT, int DH, bool VEC>
 __global__ __launch_bounds__(512) void attention_rows_kernel(BlockAttnArgs p, SeqTable t) {
   using T = typename ElemOf<DT>::T;
@@ -848,6 +852,11 @@ __global__ __launch_bounds__(kCountThreads) void scatter_entries_kernel(BlockAtt
 // the tile's entries on their own, the next ones' queries on their way. S^T =
 // K Q^T leaves a lane the scores of one query with keys 4 lg .. + 4 of every 16,
 // which is the operand of O^T = V^T P^T as it stands.
+//
+// 8,195 queries of 20 heads, 16 blocks of 64 keys each, 43 GFLOP, run in five groups
+// of heads: 65 us a group here (395 TFLOP/s of fp16 work, three products a fp32 one;
+// softmax and splits on the VALU beside it, and 138 MB of parts written), 26 joining
+// them, 40 for all the lists.
 //
 // ONE: no block is longer than 64 keys.
 template <int DT, int DH, bool VEC, bool ONE>

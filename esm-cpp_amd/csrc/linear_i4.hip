@@ -154,7 +154,9 @@ __device__ __forceinline__ void split_scaled(const float (&x)[8], uint4 (&out)[P
 // lane, 16 lanes would do one row's work over again: 1 x 10,240 x 2,560 13 us
 // instead of 8), while the first tile's codes and scales are on their way; a
 // tile's are loaded while the tile before is computed. D = W x^T, so that a
-// lane's outputs are four consecutive ones of one row.
+// lane's outputs are four consecutive ones of one row. 1 x 1,280 x 1,280 takes 4 us,
+// a launch and two trips to memory; 14 MB of 10,240 x 2,560 9, at 1.6 TB/s, a wave's
+// two tiles one after the other.
 template <int DT, int NT, int GJ>  // GJ: 32-input steps of a group within a tile (1, 2 or 4)
 __global__ __launch_bounds__(1024) void linear_i4_rows_kernel(LinearI4Args p, int chunk) {
   using T = typename Elem<DT>::T;
