@@ -316,7 +316,10 @@ __global__ __launch_bounds__(256) void linear_i4_split_kernel(LinearI4Args p, ui
 // each tile's loads and leave the CU to two or three other workgroups meanwhile
 // (67 fp32 rows of 3,840 x 1,280 11.1 us a call, 14.5 with the next tile's loads in
 // flight and one workgroup a CU); 32 x 64 ones (one plane only) have those in flight.
-// in_place: planes are the caller's fp16 rows, not the split kernel's.
+// in_place: planes are the caller's fp16 rows, not the split kernel's. A load then
+// takes 256 bytes of four rows, and a wave turns its tile round through its own
+// part of LDS (301 rows of 1,280 x 5,120 14.1 us; loaded in the operands' places,
+// four neighbouring lanes in four rows, 16.5).
 template <int DT, int MT, int NT, int GJ>
 __global__ __launch_bounds__(512, NT == 2 ? 4 : 2) void linear_i4_mid_kernel(
     LinearI4Args p, const uint16_t* planes, const float* inv, int ldp, bool in_place) {
@@ -332,9 +335,8 @@ __global__ __launch_bounds__(512, NT == 2 ? 4 : 2) void linear_i4_mid_kernel(
   const uint16_t* rows[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
-    rows[mt] = planes + (rowwise ? static_cast<size_t>(min(m0 + 16 * mt + lr, p.M - 1)) * ldp + 8 * kq
+    rows[mt] = planes + (rowwise ? static_cast<size_t>(m0 + 16 * mt) * ldp + 8 * lr
                                  : static_cast<size_t>(min(m0 / 16 + mt, (p.M - 1) / 16)) * 16 * ldp + 8 * lane);
-  const size_t step = rowwise ? 32 : 512;  // elements from 32 inputs to the next 32
   const size_t plane = plane_elems(p.M, ldp);
   struct Tile {
     u32x4 w[NT];
@@ -358,7 +360,9 @@ __global__ __launch_bounds__(512, NT == 2 ? 4 : 2) void linear_i4_mid_kernel(
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int pl = 0; pl < PL; ++pl)
-          t.a[mt][j][pl] = *reinterpret_cast<const f16x8*>(rows[mt] + pl * plane + (kt * 4 + j) * step);
+          t.a[mt][j][pl] = *reinterpret_cast<const f16x8*>(
+              rowwise ? rows[mt] + min(4 * j + kq, p.M - 1 - m0 - 16 * mt) * static_cast<ptrdiff_t>(ldp) + kt * kTileK
+                      : rows[mt] + pl * plane + (static_cast<size_t>(kt) * 4 + j) * 512);
   };
   f32x4 total[NT][MT];
 #pragma unroll
@@ -369,7 +373,24 @@ __global__ __launch_bounds__(512, NT == 2 ? 4 : 2) void linear_i4_mid_kernel(
   if (kAhead && wave < p.tiles_k) load(wave, next);
   for (int kt = wave; kt < p.tiles_k; kt += waves) {
     if (!kAhead) load(kt, next);
-    const Tile t = next;
+    Tile t = next;
+    if (rowwise) {  // row 4 j + kq, inputs 8 lr .. + 8 to row lr, inputs 32 j + 8 kq .. + 8
+      uint8_t* own = reinterpret_cast<uint8_t*>(red) + wave * (MT * 4096);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<f16x8*>(own + mt * 4096 + (4 * j + kq) * 256 + (lr ^ (4 * j + kq)) * 16) = t.a[mt][j][0];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          t.a[mt][j][0] = *reinterpret_cast<const f16x8*>(own + mt * 4096 + lr * 256 + ((4 * j + kq) ^ lr) * 16);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
     if (kAhead && kt + waves < p.tiles_k) load(kt + waves, next);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -392,6 +413,7 @@ __global__ __launch_bounds__(512, NT == 2 ? 4 : 2) void linear_i4_mid_kernel(
       }
     }
   }
+  if (rowwise) __syncthreads();  // the waves' rows lie where the sums go
   f32x4* out4 = reinterpret_cast<f32x4*>(red);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -609,7 +631,7 @@ void launch_mid(const LinearI4Args& p, const LinearI4Plan& plan, const uint16_t*
                 hipStream_t s) {
   const unsigned grid =
       static_cast<unsigned>((p.N + 16 * NT - 1) / (16 * NT)) * ((p.M + 16 * MT - 1) / (16 * MT));
-  const size_t lds = static_cast<size_t>(plan.waves) * NT * MT * 1024;
+  const size_t lds = static_cast<size_t>(plan.waves) * MT * std::max(NT * 1024, DT == kTypeF16 ? 4096 : 0);
   linear_i4_mid_kernel<DT, MT, NT, GJ><<<grid, 64 * plan.waves, lds, s>>>(p, planes, inv, ldp, plan.scratch_bytes == 0);
 }
 
@@ -657,8 +679,9 @@ LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type) {
   LinearI4Plan plan;
   const size_t tiles_n = (static_cast<size_t>(p.N) + kTileN - 1) / kTileN, cus = std::max(1, device_cus());
   // Rows that the kernels can read in place need no scratch, and no launch that
-  // splits them: then 9 rows are already better off without LDS (16 fp16 rows of
-  // 1,280 x 5,120 10.4 us split in the kernel, 8.6 read in place).
+  // splits them: then 9 rows are already better off with a workgroup for each 32 columns' share
+  // of the inputs (16 fp16 rows of 1,280 x 5,120 10.4 us split in the kernel, 67 read
+  // in place 7.3).
   const bool in_place = type == kTypeF16 && p.vec_a && p.K % kTileK == 0;
   if (p.M <= (in_place ? 8 : 16)) {
     plan.form = LinearI4Plan::kRows;
@@ -683,7 +706,7 @@ LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type) {
   // those. So 67 fp32 rows of 3,840 x 1,280 take small tiles (11 us, as a GEMM 40),
   // 256 too (23, 42), 512 of 1,280 x 5,120 as well (40, 90) and 256 of 10,240 x
   // 2,560 are a GEMM (54, in small tiles 58); 301 fp16 rows of 1,280 x 5,120 take
-  // wide tiles (16, small ones 21, as a GEMM 57).
+  // wide tiles (14, as a GEMM 57).
   const bool two = type == kTypeF32, g32 = p.group == 32;
   auto tiles = [](int n, int by) { return (n + by - 1.0) / by; };
   const auto wgs = [&](int rows, int cols) { return std::floor(tiles(p.M, rows)) * std::floor(tiles(p.N, cols)); };
