@@ -146,6 +146,7 @@ struct esm_gfx950_weight {
 
 struct esm_gfx950_weight_i4 {
   int N = 0, K = 0, group = 0, groups = 0, tiles_k = 0;
+  int device = 0;
   uint32_t* codes = nullptr;  // linear_i4_layout's order
   float* scales = nullptr;
 };
@@ -928,6 +929,7 @@ extern "C" int esm_gfx950_weight_upload_i4(esm_gfx950_ctx* ctx, const uint8_t* p
     w->N = N;
     w->K = K;
     w->group = group;
+    w->device = ctx->device;
     w->groups = (K - 1) / group + 1;
     w->tiles_k = static_cast<int>(tiles_k);
     std::vector<uint32_t> codes(tiles_n * tiles_k * 256);
@@ -973,12 +975,15 @@ extern "C" int esm_gfx950_linear_i4(esm_gfx950_ctx* ctx, const void* A, int lda,
   ESM_REQUIRE(ctx, W && M >= 0, "linear_i4: bad arguments");
   if (W->N != N || W->K != K)
     return ctx->fail(ESM_GFX950_SHAPE_MISMATCH, "linear_i4: weight shape does not match N, K");
+  ESM_REQUIRE(ctx, W->device == ctx->device, "linear_i4: the weight lies on another GPU");
   if (M == 0) return ESM_GFX950_OK;
   ESM_REQUIRE(ctx, A && C, "linear_i4: null pointer");
   ESM_REQUIRE(ctx, lda >= K && ldc >= N, "linear_i4: lda must be >= K and ldc >= N");
   ESM_REQUIRE(ctx, aligned(A, size) && aligned(C, size) && aligned(bias, 4), "linear_i4: misaligned pointer");
-  ESM_REQUIRE(ctx, !bytes_overlap(A, span_bytes(M, lda, K, size), C, span_bytes(M, ldc, N, size)),
-              "linear_i4: C shares memory with A");
+  const size_t c_bytes = span_bytes(M, ldc, N, size);
+  ESM_REQUIRE(ctx, !bytes_overlap(A, span_bytes(M, lda, K, size), C, c_bytes), "linear_i4: C shares memory with A");
+  ESM_REQUIRE(ctx, !bias || !bytes_overlap(bias, static_cast<size_t>(N) * 4, C, c_bytes),
+              "linear_i4: C shares memory with bias");
   DeviceScope on(ctx);
   LinearI4Args p;
   p.A = A;

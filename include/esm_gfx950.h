@@ -259,7 +259,8 @@ int esm_gfx950_weight_free_i4(esm_gfx950_ctx* ctx, esm_gfx950_weight_i4* w);
  * quantised: products take fp16 and bf16 ones as they are and 22 significant
  * bits of fp32 ones (bf16 and fp32 ones to 2^-39 of the row's largest input where
  * that is coarser), sums are fp32, rounded once to dtype. C must not share memory
- * with A. M == 0 is a no-op. N and K must be the weight's (SHAPE_MISMATCH).
+ * with A or bias. M == 0 is a no-op. N and K must be the weight's
+ * (SHAPE_MISMATCH), and the weight on the context's GPU.
  * Scratch for the split rows (up to 4 M K bytes) stays with the context. */
 int esm_gfx950_linear_i4(esm_gfx950_ctx* ctx, const void* A, int lda, const esm_gfx950_weight_i4* W,
                          const float* bias, void* C, int ldc, int M, int N, int K, int dtype);

@@ -298,3 +298,15 @@ def test_refusals(dev):
     refused(eg.INVALID_ARGUMENT, At(A, 2), W, None, C, 3, 4, 16)
     dev.linear_i4(A, W, None, C, 0, 4, 16)  # no rows: nothing to do
     W.free()
+
+
+def test_outputs_over_the_bias_are_refused(dev):
+    """The bias is read while other outputs are written."""
+    W = dev.weight_i4(np.zeros((4, 8), np.uint8), np.zeros((4, 1), np.float32), 16, 32)
+    A, C = dev.array(np.zeros((4, 16), np.float32)), dev.array(np.zeros(64, np.float32))
+    with pytest.raises(eg.Gfx950Error) as e:
+        dev.linear_i4(A, W, At(C, 15 * 4), C, 4, 4, 16)
+    assert e.value.code == eg.INVALID_ARGUMENT
+    dev.linear_i4(A, W, At(C, 16 * 4), C, 4, 4, 16)
+    assert (C.numpy() == 0).all()
+    W.free()
