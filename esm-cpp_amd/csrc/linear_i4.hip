@@ -696,26 +696,33 @@ LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type) {
     return plan;
   }
   const int ldp = in_place ? p.lda : p.tiles_k * kTileK;
-  // The call's time on an idle device, in us, as measured over 17 to 512 rows of
-  // 1,280 x 1,280, 3,840 x 1,280, 5,120 x 1,280, 1,280 x 5,120 and 10,240 x 2,560,
-  // the rows' split left out: small tiles 1 for each 128-input tile of a wave and, as
-  // the CUs hold two or three, 0.15 (two planes and groups of 32: 0.2) for each of a
-  // CU's; wide ones 3 for each of a wave's in each round of one workgroup per CU; a
-  // GEMM workgroup 10 and 0.6 (two planes 0.97, groups of 32 0.4 more) per 64 inputs
-  // while it has a CU to itself, 1.4 times that where two share one, and rounds of
-  // those. So 67 fp32 rows of 3,840 x 1,280 take small tiles (11 us, as a GEMM 40),
-  // 256 too (23, 42), 512 of 1,280 x 5,120 as well (40, 90) and 256 of 10,240 x
-  // 2,560 are a GEMM (54, in small tiles 58); 301 fp16 rows of 1,280 x 5,120 take
-  // wide tiles (14, as a GEMM 57).
+  // The call's time on an idle device, in us, as measured over 17 to 4,096 rows of
+  // 1,280 x 1,280, 3,840 x 1,280, 1,280 x 5,120, 2,560 x 2,560, 10,240 x 2,560 and
+  // 2,560 x 10,240, the rows' split left out: small tiles 1 for each 128-input tile of
+  // a wave and, as the CUs hold two or three, 0.5 (groups of 32: 0.75, turned round
+  // 1.75) and 0.08 (two planes 0.12, groups of 32 0.03 more) per 128 inputs for each
+  // of a CU's; wide ones 1.5 and 2.3 for each tile of a wave in each round of one
+  // workgroup per CU; a GEMM workgroup 10 and 0.6 (two planes 0.97, groups of 32 0.5
+  // more) per 64 inputs while it has a CU to itself, 1.4 times that where two share
+  // one, and rounds of those (groups of 32 leave registers for one only). So 67 fp32
+  // rows of 3,840 x 1,280 take small tiles (11 us, as a GEMM 40), 256 too (23, 42), 512
+  // of 1,280 x 5,120 as well (40, 90) and 400 of 10,240 x 2,560 are a GEMM (76, in
+  // small tiles 84); 301 fp16 rows of 1,280 x 5,120 take wide tiles (14, as a GEMM 57),
+  // 256 of 2,560 x 10,240 small ones (40, wide 44).
   const bool two = type == kTypeF32, g32 = p.group == 32;
   auto tiles = [](int n, int by) { return (n + by - 1.0) / by; };
   const auto wgs = [&](int rows, int cols) { return std::floor(tiles(p.M, rows)) * std::floor(tiles(p.N, cols)); };
   const int iterations = (p.tiles_k + 7) / 8;
   const double gemm_wgs = wgs(kGemmM, kGemmN);
-  const double small_us = iterations + (two && g32 ? 0.2 : 0.15) * p.tiles_k * wgs(16, 32) / cus;
-  const double wide_us = two || g32 ? 1e30 : 3.0 * iterations * std::ceil(wgs(32, 64) / cus);
-  const double gemm_us = (10.0 + ((two ? 0.97 : 0.6) + (g32 ? 0.4 : 0.0)) * 2 * p.tiles_k) *
-                         (gemm_wgs <= cus ? 1.0 : 1.4 * std::max(1.0, gemm_wgs / (2.0 * cus)));
+  const double of32 = g32 ? 1.0 : 0.0;
+  const double small_each =
+      0.5 + (in_place ? 1.25 : 0.25) * of32 + ((two ? 0.12 : 0.08) + 0.03 * of32) * p.tiles_k;
+  const double small_us = iterations + small_each * wgs(16, 32) / cus;
+  const double wide_us = two || g32 ? 1e30 : (1.5 + 2.3 * iterations) * std::ceil(wgs(32, 64) / cus);
+  const double gemm_rounds = gemm_wgs <= cus ? 1.0
+                             : g32           ? std::ceil(gemm_wgs / cus)
+                                             : 1.4 * std::max(1.0, gemm_wgs / (2.0 * cus));
+  const double gemm_us = (10.0 + ((two ? 0.97 : 0.6) + 0.5 * of32) * 2 * p.tiles_k) * gemm_rounds;
   // A GEMM tile's 64 rows are 32-bit offsets apart, and its grid is one number.
   const bool gemm_ok = ldp < (1 << 23) && gemm_wgs < 2e9;
   plan.wide = wide_us < small_us;
