@@ -355,7 +355,7 @@ struct LinearI4Args {
   int tiles_k = 0;  // ceil(K / 128)
   bool vec_a = false;  // A's rows start at 16-byte addresses
 };
-// How linear_i4 runs: few rows (up to 16, or 8 that need no splitting) with the
+// How linear_i4 runs: few rows (up to 16, or 4 that need no splitting) with the
 // activations split in the kernel, or on activations split into scratch
 // beforehand, in small tiles with the inputs spread over the waves or as a GEMM.
 struct LinearI4Plan {

@@ -679,13 +679,20 @@ LinearI4Plan linear_i4_plan(const LinearI4Args& p, int type) {
   LinearI4Plan plan;
   const size_t tiles_n = (static_cast<size_t>(p.N) + kTileN - 1) / kTileN, cus = std::max(1, device_cus());
   // Rows that the kernels can read in place need no scratch, and no launch that
-  // splits them: then 9 rows are already better off with a workgroup for each 32 columns' share
-  // of the inputs (16 fp16 rows of 1,280 x 5,120 10.4 us split in the kernel, 67 read
-  // in place 7.3).
+  // splits them (16 fp16 rows of 1,280 x 5,120 10.4 us split in the kernel, 7.0 read
+  // in place). Splitting in every workgroup costs about 0.025 us a row and 128 inputs
+  // on each CU, small tiles one more launch: 10 fp32 rows of 1,280 x 1,280 take 5.0
+  // us split in the kernel (7.7 the other way), 13 of 1,280 x 5,120 13 (15), 8 of
+  // 10,240 x 2,560 11 (14).
   const bool in_place = type == kTypeF16 && p.vec_a && p.K % kTileK == 0;
-  if (p.M <= (in_place ? 8 : 16)) {
+  const bool pairs = tiles_n >= 2 * cus && p.group != 32;  // two with four groups a tile spill
+  const double row_cus = std::max(1.0, static_cast<double>(pairs ? tiles_n / 2 : tiles_n) / cus);
+  const double tiles_us = (p.tiles_k + 7) / 8 + (0.5 + 0.12 * p.tiles_k) * (tiles_n / 2) / cus + 5.5;
+  const double rows_us = 2.7 + 3.3e-3 * (p.group == 32 ? 1.7 : 1.0) * tiles_n * p.tiles_k / 8 +
+                         0.025 * p.tiles_k * p.M * row_cus;
+  if (p.M <= 4 || (p.M <= 16 && !in_place && rows_us <= tiles_us)) {
     plan.form = LinearI4Plan::kRows;
-    plan.col_tiles = tiles_n >= 2 * cus && p.group != 32 ? 2 : 1;  // two with four groups a tile spill
+    plan.col_tiles = pairs ? 2 : 1;
     // As many waves as give each the same number of tiles, at most 10, and as many
     // of the waves' tiles at a time as keep the activations in 60 KB of LDS.
     const int rounds = (p.tiles_k + 9) / 10;
